@@ -95,12 +95,13 @@ class Lib:
         return n.value if st == 0 else 0
 
     # -- device arrays ---------------------------------------------------------------------
-    def empty(self, shape, dev=0):
-        return DeviceArray(self, tuple(np.atleast_1d(shape)) if not isinstance(shape, tuple) else shape, dev)
+    def empty(self, shape, dev=0, dtype=np.float32):
+        return DeviceArray(self, tuple(np.atleast_1d(shape)) if not isinstance(shape, tuple) else shape, dev, dtype)
 
-    def to_device(self, arr, dev=0):
-        arr = np.ascontiguousarray(arr, dtype=np.float32)
-        d = DeviceArray(self, arr.shape, dev)
+    def to_device(self, arr, dev=0, dtype=np.float32):
+        """A copy on the device, as fp32 unless another type is asked for (int32 class numbers, uint8 for values in 8 bits)."""
+        arr = np.ascontiguousarray(arr, dtype=dtype)
+        d = DeviceArray(self, arr.shape, dev, dtype)
         if arr.size:
             self.call("memcpy_h2d", dev, d.ptr, arr.ctypes.data_as(ctypes.c_void_p), arr.nbytes)
         return d
@@ -121,17 +122,18 @@ class Lib:
 
 
 class DeviceArray:
-    """fp32 device buffer owned through eddlb200_alloc / eddlb200_free."""
+    """Device buffer owned through eddlb200_alloc / eddlb200_free; fp32 unless another numpy type is given."""
 
-    def __init__(self, lib, shape, dev=0):
+    def __init__(self, lib, shape, dev=0, dtype=np.float32):
         self.lib, self.shape, self.dev = lib, tuple(int(s) for s in shape), dev
         self.size = int(np.prod(self.shape)) if len(self.shape) else 1
+        self.dtype = np.dtype(dtype)
         p = ctypes.c_void_p()
-        lib.call("alloc", dev, max(self.size, 1) * 4, ctypes.byref(p))
+        lib.call("alloc", dev, max(self.size, 1) * self.dtype.itemsize, ctypes.byref(p))
         self.ptr, self.addr = p, p.value
 
     def numpy(self):
-        out = np.empty(self.shape, dtype=np.float32)
+        out = np.empty(self.shape, dtype=self.dtype)
         if self.size:
             self.lib.call("memcpy_d2h", self.dev, out.ctypes.data_as(ctypes.c_void_p), self.ptr, out.nbytes)
         return out

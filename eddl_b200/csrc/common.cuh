@@ -41,6 +41,8 @@ ncclComm *comm_of(DevCtx *c);
 int comm_nranks(DevCtx *c);
 void count_launch(DevCtx *c, unsigned n = 1);
 int set_error(int code, const char *fmt, ...);
+// Reads and clears the device's time-out flag of the 8-bit products (blocking; nothing is read on a device that has run none).
+int fp8_status(int dev, cudaStream_t st, int *out);
 
 // Optional per-kernel-family device timing (CUDA events on the compute stream), off by
 // default.  `work` is the family's algorithmic work of this call (FLOPs or bytes).
@@ -225,6 +227,19 @@ inline void launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cud
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t c = {};
     c.gridDim = grid; c.blockDim = block; c.dynamicSmemBytes = smem; c.stream = st; c.attrs = at; c.numAttrs = 1;
+    cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
+
+// The same with clusters of `cluster` blocks along x (at most eight: every device of this architecture holds those).
+template <typename... P, typename... A>
+inline void launch_cluster(void (*kernel)(P...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A &&...args) {
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid; c.blockDim = block; c.dynamicSmemBytes = smem; c.stream = st; c.attrs = at; c.numAttrs = 2;
     cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
 }
 

@@ -1,0 +1,489 @@
+// Dense algebra in 8-bit floating point with an fp32 scale for each block of 128 values along the reduction: quantisation of a
+// tensor in both of its directions, and the product of two quantised matrices on the tensor cores.
+#include <cuda_fp8.h>
+#include "tc_ptx.cuh"
+
+namespace {
+
+using namespace eb;
+
+constexpr int kBlk = 128;
+
+// ---- quantisation ------------------------------------------------------------------------------------------------------------
+// One block per 128 x 128 tile, one read of it for both directions; bound by memory (4 bytes read, 1 or 2 written a value).  A warp
+// takes 16 rows, a lane four columns of each, so a row's 128 values are one 512-byte access and their largest magnitude one warp
+// reduction; the columns' come from the warps' through shared memory.  The transpose goes through a 16 KB byte tile (16-byte pieces,
+// swizzled so that neither side has bank conflicts) and leaves in 128-byte lines.
+struct QuantArgs {
+    const float *a;
+    uint8_t *q, *qt;
+    float *scale, *scale_t;
+    size_t ldq, ldqt;
+    int rows, cols, tiles_x;
+    int pow2;
+};
+
+struct Scale { float scale, factor; };
+template <int FORMAT>
+__device__ __forceinline__ Scale scale_of(unsigned peak_bits, int pow2) {
+    constexpr float largest = FORMAT == EDDLB200_E4M3 ? 448.f : 57344.f;
+    constexpr unsigned least = 27u << 23;                              // 2^-100
+    const float peak = __uint_as_float(max(peak_bits, least));
+    if (peak_bits >= 0x7f800000u) return Scale{__uint_as_float(0x7f800000u), 0.f};
+    if (!pow2) return Scale{__fdiv_rn(peak, largest), __fdiv_rn(largest, peak)};
+    // both formats' largest number is 1.75 2^E: the power is the peak's own, one more where its mantissa is past 1.75
+    constexpr int E = FORMAT == EDDLB200_E4M3 ? 8 : 15;
+    const unsigned bits = __float_as_uint(peak);
+    const int power = (int)(bits >> 23) - 127 - E + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return Scale{__uint_as_float((unsigned)(power + 127) << 23), __uint_as_float((unsigned)(127 - power) << 23)};
+}
+template <int FORMAT>
+__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
+    constexpr __nv_fp8_interpretation_t kind = FORMAT == EDDLB200_E4M3 ? __NV_E4M3 : __NV_E5M2;
+    const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, kind), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, kind);
+    return lo | hi << 16;
+}
+// magnitude as bits, in which larger numbers are larger; a NaN counts as nothing
+__device__ __forceinline__ unsigned magnitude(float v) { const unsigned b = __float_as_uint(v) & 0x7fffffffu; return b > 0x7f800000u ? 0u : b; }
+
+template <int FORMAT, bool TILE, bool VEC>
+__global__ void __launch_bounds__(256, 2) fp8_quantize_kernel(const QuantArgs a) {
+    EB_GRID_WAIT();
+    __shared__ unsigned col_peak[8][kBlk];
+    __shared__ __align__(16) uint8_t turned[kBlk * kBlk];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tx = blockIdx.x % a.tiles_x, ty = blockIdx.x / a.tiles_x;
+    const int r0 = ty * kBlk + warp * 16, c0 = tx * kBlk + lane * 4;
+    float v[16][4];
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const float *src = a.a + (size_t)(r0 + i) * a.cols + c0;
+        const bool row = r0 + i < a.rows;
+        if (VEC) {
+            const float4 q = row && c0 < a.cols ? ld_stream4(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[i][j] = row && c0 + j < a.cols ? src[j] : 0.f;
+        }
+    }
+    unsigned mine[4] = {0, 0, 0, 0};                                   // of the lane's columns over the warp's rows
+    if (TILE || a.qt) {
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) mine[j] = max(mine[j], magnitude(v[i][j]));
+        *reinterpret_cast<uint4 *>(&col_peak[warp][lane * 4]) = make_uint4(mine[0], mine[1], mine[2], mine[3]);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            const uint4 p = *reinterpret_cast<const uint4 *>(&col_peak[w][lane * 4]);
+            mine[0] = max(mine[0], p.x); mine[1] = max(mine[1], p.y); mine[2] = max(mine[2], p.z); mine[3] = max(mine[3], p.w);
+        }
+    }
+    Scale tile{0.f, 0.f};
+    if (TILE) {
+        tile = scale_of<FORMAT>(__reduce_max_sync(0xffffffffu, max(max(mine[0], mine[1]), max(mine[2], mine[3]))), a.pow2);
+        if (threadIdx.x == 0) {
+            const int row_blocks = (a.rows + kBlk - 1) / kBlk;
+            if (a.q) a.scale[(size_t)tx * row_blocks + ty] = tile.scale;
+            if (a.qt) a.scale_t[(size_t)ty * a.tiles_x + tx] = tile.scale;
+        }
+    }
+    if (a.q) {
+        float own_scale = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            Scale s = tile;
+            if (!TILE) {
+                s = scale_of<FORMAT>(__reduce_max_sync(0xffffffffu, max(max(magnitude(v[i][0]), magnitude(v[i][1])), max(magnitude(v[i][2]), magnitude(v[i][3])))), a.pow2);
+                if (lane == i) own_scale = s.scale;
+            }
+            if (r0 + i >= a.rows || c0 >= a.cols) continue;
+            const unsigned bytes = pack4<FORMAT>(__fmul_rn(v[i][0], s.factor), __fmul_rn(v[i][1], s.factor), __fmul_rn(v[i][2], s.factor), __fmul_rn(v[i][3], s.factor));
+            uint8_t *dst = a.q + (size_t)(r0 + i) * a.ldq + c0;
+            if (VEC || c0 + 4 <= a.cols) *reinterpret_cast<unsigned *>(dst) = bytes;
+            else for (int j = 0; c0 + j < a.cols; j++) dst[j] = (uint8_t)(bytes >> 8 * j);
+        }
+        if (!TILE && lane < 16 && r0 + lane < a.rows) a.scale[(size_t)tx * a.rows + r0 + lane] = own_scale;
+    }
+    if (!a.qt) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        Scale s = tile;
+        if (!TILE) {
+            s = scale_of<FORMAT>(mine[j], a.pow2);
+            if (warp == 0 && c0 + j < a.cols) a.scale_t[(size_t)ty * a.cols + c0 + j] = s.scale;
+        }
+        unsigned b[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            b[i] = pack4<FORMAT>(__fmul_rn(v[4 * i][j], s.factor), __fmul_rn(v[4 * i + 1][j], s.factor), __fmul_rn(v[4 * i + 2][j], s.factor), __fmul_rn(v[4 * i + 3][j], s.factor));
+        *reinterpret_cast<uint4 *>(turned + (lane * 4 + j) * kBlk + ((warp ^ lane) & 7) * 16) = make_uint4(b[0], b[1], b[2], b[3]);
+    }
+    __syncthreads();
+    const int at = (threadIdx.x & 7) * 16, left = a.rows - ty * kBlk - at;            // bytes of this piece that are there
+    if (left <= 0) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int col = (int)(threadIdx.x >> 3) + 32 * i, gc = tx * kBlk + col;
+        if (gc >= a.cols) break;
+        const uint8_t *src = turned + col * kBlk + (((threadIdx.x & 7) ^ (col >> 2)) & 7) * 16;
+        uint8_t *dst = a.qt + (size_t)gc * a.ldqt + (size_t)ty * kBlk + at;
+        if (left >= 16) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+        else for (int j = 0; j < left; j++) dst[j] = src[j];
+    }
+}
+
+template <int FORMAT>
+auto quantize_kernel(bool tile, bool vec) {
+    return tile ? (vec ? fp8_quantize_kernel<FORMAT, true, true> : fp8_quantize_kernel<FORMAT, true, false>)
+                : (vec ? fp8_quantize_kernel<FORMAT, false, true> : fp8_quantize_kernel<FORMAT, false, false>);
+}
+
+// ---- product -----------------------------------------------------------------------------------------------------------------
+// D[i][j] = sum over blocks b: s_i[b] s_j[b] sum_k P[i][k] Q[j][k].  The tensor core's M side (128 lanes of tensor memory) is the matrix whose rows are
+// C's COLUMNS, so that the lanes of a warp store to neighbouring addresses, and its N side the one whose rows are C's rows: BN of
+// them, as few as 16 for a single token.  Every K-block of 128 is one accumulation of four instructions into tensor memory; the
+// epilogue warps take it out, scale it and add it to fp32 sums in registers while the next K-block runs into the other buffer.
+// Where the tiles do not fill the GPU a cluster of up to eight blocks shares the K-blocks of a tile and adds its partial
+// tiles in rank order through distributed shared memory: one launch, no partial sums in memory.
+struct ProdParams {
+    CUtensorMap map_p, map_q;
+    const float *scale_p, *scale_q;
+    float *c;
+    int p_rows, q_rows, kblocks;             // p_rows: columns of C, q_rows: rows of C
+    int p_shift, q_shift, p_scales, q_scales;   // rows of a scale (log2) and scales of a K-block
+    int tiles_p, splits, inc;
+    unsigned idesc;
+};
+
+// site of the first wait that gave up | warp << 8 | 6 << 16; 0 = none since the last look
+__device__ int g_fp8_status;
+bool g_fp8_used[EDDLB200_MAX_DEVICES] = {};
+
+template <int BN>
+struct ProdShape {
+    static constexpr int EPI = BN >= 64 ? 8 : 4, THREADS = 64 + EPI * 32, COLS = BN / (EPI / 4);
+    static constexpr int STAGE = 128 * kBlk + BN * kBlk, STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
+    static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int PER_LANE = (COLS + 31) / 32;
+    static constexpr int SCALES = EPI * 2 * PER_LANE * 32 * 4;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES;
+    static_assert(STAGES * STAGE >= BN * 512, "the partial tile of a split takes the place of the operands");
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst_smem), "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void umma_fp8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// fp32 sums, both operands K-major; formats: 0 = e4m3, 1 = e5m2
+constexpr unsigned fp8_idesc(int format_a, int format_b, int m, int n) {
+    return (1u << 4) | (unsigned)format_a << 7 | (unsigned)format_b << 10 | (unsigned)(n >> 3) << 17 | (unsigned)(m >> 4) << 24;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(ProdShape<BN>::THREADS, 1) fp8_product_kernel(const __grid_constant__ ProdParams P) {
+    using S = ProdShape<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float *scales = (float *)(ring + S::STAGES * S::STAGE);
+    __shared__ __align__(8) uint64_t bars[2 * S::STAGES + 4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES, bar_acc_full = bar_empty + 8 * S::STAGES, bar_acc_empty = bar_acc_full + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)(blockIdx.x % P.splits), tile = (int)(blockIdx.x / P.splits);
+    const int p0 = (tile % P.tiles_p) * 128, q0 = (tile / P.tiles_p) * BN;
+    const int kb0 = (int)((long long)P.kblocks * split / P.splits), kb1 = (int)((long long)P.kblocks * (split + 1) / P.splits);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; s++) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
+        for (int s = 0; s < 2; s++) { mbar_init(bar_acc_full + 8 * s, 1); mbar_init(bar_acc_empty + 8 * s, S::EPI); }
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), S::TMEM);
+    EB_GRID_WAIT();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    int fail = 0;
+    float acc[S::COLS];
+#pragma unroll
+    for (int i = 0; i < S::COLS; i++) acc[i] = 0.f;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;              // of an epilogue warp
+
+    if (warp == 0) {
+        // ============================ copies ============================
+        if (elect_one()) {
+            int s = 0; uint32_t phase = 1;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!mbar_wait(bar_empty + 8 * s, phase, abort_flag)) { fail = 1; break; }
+                mbar_expect_tx(bar_full + 8 * s, S::STAGE);
+                const uint32_t dst = smem_u32(ring) + s * S::STAGE;
+                tma_load_2d(dst, &P.map_p, kb * kBlk, p0, bar_full + 8 * s);
+                tma_load_2d(dst + 128 * kBlk, &P.map_q, kb * kBlk, q0, bar_full + 8 * s);
+                if (++s == S::STAGES) { s = 0; phase ^= 1u; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ============================ MMA issue ============================
+        if (elect_one()) {
+            int s = 0, buf = 0; uint32_t phase = 0, acc_phase = 1;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!mbar_wait(bar_acc_empty + 8 * buf, acc_phase, abort_flag)) { fail = 2; break; }
+                if (!mbar_wait(bar_full + 8 * s, phase, abort_flag)) { fail = 3; break; }
+                tc_fence_after();
+                const uint64_t pd = make_desc(smem_u32(ring) + s * S::STAGE), qd = make_desc(smem_u32(ring) + s * S::STAGE + 128 * kBlk);
+#pragma unroll
+                for (int k = 0; k < 4; k++) umma_fp8(tmem + buf * BN, pd + 2 * k, qd + 2 * k, P.idesc, k ? 1u : 0u);
+                umma_commit(bar_empty + 8 * s);
+                umma_commit(bar_acc_full + 8 * buf);
+                if (++s == S::STAGES) { s = 0; phase ^= 1u; }
+                if (++buf == 2) { buf = 0; acc_phase ^= 1u; }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ============================ epilogue ============================
+        float *mine = scales + (warp - 2) * (2 * S::PER_LANE * 32);
+        const int p = p0 + quarter * 32 + lane, q = q0 + half * S::COLS;
+        const float *sp = P.scale_p + min(p, P.p_rows - 1) / (1 << P.p_shift);
+        float next_p = 0.f, next_q[S::PER_LANE];
+        auto fetch = [&](int kb) {
+            if (kb >= kb1) return;
+            next_p = __ldg(sp + (size_t)kb * P.p_scales);
+#pragma unroll
+            for (int i = 0; i < S::PER_LANE; i++) {
+                const int row = q + i * 32 + lane;
+                next_q[i] = row < P.q_rows ? __ldg(P.scale_q + (size_t)kb * P.q_scales + (row >> P.q_shift)) : 0.f;
+            }
+        };
+        fetch(kb0);
+        int buf = 0; uint32_t phase = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            float *line = mine + (buf * S::PER_LANE) * 32;
+#pragma unroll
+            for (int i = 0; i < S::PER_LANE; i++) line[i * 32 + lane] = next_q[i];
+            const float s_p = next_p;
+            __syncwarp();
+            fetch(kb + 1);
+            if (!mbar_wait_warp(bar_acc_full + 8 * buf, phase, abort_flag)) { fail = 4; break; }
+            tc_fence_after();
+            const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN + half * S::COLS);
+#pragma unroll
+            for (int c = 0; c < S::COLS; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(base + c, r);
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 s4 = *reinterpret_cast<const float4 *>(line + c + j);
+                    acc[c + j] = fmaf(__uint_as_float(r[j]) * s4.x, s_p, acc[c + j]);
+                    acc[c + j + 1] = fmaf(__uint_as_float(r[j + 1]) * s4.y, s_p, acc[c + j + 1]);
+                    acc[c + j + 2] = fmaf(__uint_as_float(r[j + 2]) * s4.z, s_p, acc[c + j + 2]);
+                    acc[c + j + 3] = fmaf(__uint_as_float(r[j + 3]) * s4.w, s_p, acc[c + j + 3]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_acc_empty + 8 * buf);
+            if (++buf == 2) { buf = 0; phase ^= 1u; }
+        }
+        if (P.splits == 1) {
+            float *dst = P.c + (size_t)q * P.p_rows + p;
+            if (p < P.p_rows) {
+#pragma unroll
+                for (int i = 0; i < S::COLS; i++)
+                    if (q + i < P.q_rows) {
+                        float *at = dst + (size_t)i * P.p_rows;
+                        *at = P.inc ? *at + acc[i] : acc[i];
+                    }
+            }
+        } else {
+            // every operand has been read by an MMA that has completed: the ring takes the partial tile
+            float *part = (float *)ring + (half * S::COLS) * 128 + quarter * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < S::COLS; i++) part[i * 128] = acc[i];
+        }
+    }
+    if (fail) { *abort_flag = 1; atomicCAS(&g_fp8_status, 0, fail | warp << 8 | 6 << 16); }
+    if (P.splits > 1) {
+        __syncwarp();
+        cluster_arrive(); cluster_wait();
+        if (warp >= 2) {
+            const int column = (threadIdx.x - 64) & 127, p = p0 + column;
+            for (int i = split + P.splits * ((threadIdx.x - 64) >> 7); i < BN && q0 + i < P.q_rows; i += P.splits * (S::EPI / 4)) {
+                float sum = 0.f;
+                for (int r = 0; r < P.splits; r++) {
+                    float v;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(ring) + (i * 128 + column) * 4, r)));
+                    sum += v;
+                }
+                if (p < P.p_rows) {
+                    float *at = P.c + (size_t)(q0 + i) * P.p_rows + p;
+                    *at = P.inc ? *at + sum : sum;
+                }
+            }
+        }
+        cluster_arrive(); cluster_wait();                   // a block's shared memory outlives the reads of the others
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, S::TMEM);
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                             const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// the driver entry point is looked up at run time: the library must load (and refuse work) on a machine without a driver
+EncodeFn encode_function() {
+    static const EncodeFn encode = []() -> EncodeFn {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) return (EncodeFn)fn;
+        cudaGetLastError();
+        return nullptr;
+    }();
+    return encode;
+}
+// [rows][cols] bytes as boxes of 128 columns and box_rows rows in the K-major 128-byte swizzle; what lies past either edge arrives as zeros
+bool encode_bytes_map(CUtensorMap *map, const void *base, size_t ld, int rows, int cols, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {(cuuint32_t)kBlk, (cuuint32_t)box_rows}, elem[2] = {1, 1};
+    const EncodeFn encode = encode_function();
+    return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN>
+int launch_product(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P, unsigned tiles) {
+    static bool configured[EDDLB200_MAX_DEVICES] = {};
+    using S = ProdShape<BN>;
+    if (!configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(fp8_product_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e != cudaSuccess) return cuda_status(e, "fp8_mult2d(attributes)");
+        configured[dev] = true;
+    }
+    if (P.splits > 1) eb::launch_cluster(fp8_product_kernel<BN>, (unsigned)P.splits, tiles * P.splits, S::THREADS, S::SMEM, st, P);
+    else eb::launch(fp8_product_kernel<BN>, tiles, S::THREADS, S::SMEM, st, P);
+    EB_LAUNCH_CHECK("fp8_mult2d");
+    g_fp8_used[dev] = true;
+    return 0;
+}
+
+size_t matrix_bytes(int rows, int cols, size_t ld) { return rows && cols ? (size_t)(rows - 1) * ld + cols : 0; }
+size_t scale_bytes(int rows, int cols, int block_rows) { return ceil_div(cols, kBlk) * ceil_div(rows, block_rows) * sizeof(float); }
+
+}  // namespace
+
+namespace eb {
+// 0 = no kernel of this file has given up waiting on the device since the last call
+int fp8_status(int dev, cudaStream_t st, int *out) {
+    *out = 0;
+    if (!g_fp8_used[dev]) return 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(out, g_fp8_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && *out) { const int zero = 0; e = cudaMemcpyToSymbolAsync(g_fp8_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st); }
+    return e == cudaSuccess ? 0 : (int)e;
+}
+}  // namespace eb
+
+using namespace eb;
+
+extern "C" {
+
+int eddlb200_fp8_quantize(int dev, const float *a, int rows, int cols, int format, int block_rows, int pow2,
+                          void *q, size_t ldq, float *scale, void *qt, size_t ldqt, float *scale_t) {
+    const char *what = "fp8_quantize";
+    EB_REQUIRE(rows >= 0 && cols >= 0, what);
+    EB_REQUIRE(format == EDDLB200_E4M3 || format == EDDLB200_E5M2, what);
+    EB_REQUIRE(block_rows == 1 || block_rows == kBlk, what);
+    EB_REQUIRE(pow2 == 0 || pow2 == 1, what);
+    EB_REQUIRE(q || qt, what);
+    EB_REQUIRE(!q || (scale && aligned16(q) && ldq % 16 == 0 && ldq >= (size_t)cols), what);
+    EB_REQUIRE(!qt || (scale_t && aligned16(qt) && ldqt % 16 == 0 && ldqt >= (size_t)rows), what);
+    EB_REQUIRE(!rows || !cols || a, what);
+    const size_t tiles = ceil_div(rows, kBlk) * ceil_div(cols, kBlk);
+    if (tiles > 0x7fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, rows, cols);
+    const size_t in = (size_t)rows * cols * sizeof(float);
+    const void *out[] = {q, scale, qt, scale_t};
+    const size_t bytes[] = {matrix_bytes(rows, cols, ldq), scale_bytes(rows, cols, block_rows), matrix_bytes(cols, rows, ldqt), scale_bytes(cols, rows, block_rows)};
+    for (int i = 0; i < 4; i++) {
+        if (!out[i / 2 * 2]) continue;
+        EB_REQUIRE(!overlap(out[i], bytes[i], a, in), what);
+        for (int j = 0; j < i; j++) EB_REQUIRE(!out[j / 2 * 2] || !overlap(out[i], bytes[i], out[j], bytes[j]), what);
+    }
+    EB_CTX(dev);
+    if (!rows || !cols) return 0;
+    EB_READS(a, in);
+    for (int i = 0; i < 4; i++) {
+        if (!out[i / 2 * 2]) continue;
+        if (i & 1) EB_WRITES(out[i], bytes[i]); else EB_MODIFIES(out[i], bytes[i]);           // bytes between the rows stay
+    }
+    ProfScope prof(cx, PROF_ELEMENTWISE, (double)rows * cols * (4 + (q ? 1 : 0) + (qt ? 1 : 0)));
+    const QuantArgs args{a, (uint8_t *)q, (uint8_t *)qt, scale, scale_t, ldq, ldqt, rows, cols, (int)ceil_div(cols, kBlk), pow2};
+    const bool vec = cols % 4 == 0 && aligned16(a);
+    auto kernel = format == EDDLB200_E4M3 ? quantize_kernel<EDDLB200_E4M3>(block_rows == kBlk, vec) : quantize_kernel<EDDLB200_E5M2>(block_rows == kBlk, vec);
+    eb::launch(kernel, (unsigned)tiles, 256, 0, st, args);
+    EB_LAUNCH_CHECK(what);
+    return 0;
+}
+
+int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_a, int format_a, int block_a, const void *qb, size_t ldb,
+                        const float *scale_b, int format_b, int block_b, float *c, int inc_c, int m, int n, int k) {
+    const char *what = "fp8_mult2d";
+    EB_REQUIRE(m >= 0 && n >= 0 && k >= 0, what);
+    EB_REQUIRE((format_a == EDDLB200_E4M3 || format_a == EDDLB200_E5M2) && (format_b == EDDLB200_E4M3 || format_b == EDDLB200_E5M2), what);
+    EB_REQUIRE((block_a == 1 || block_a == kBlk) && (block_b == 1 || block_b == kBlk), what);
+    EB_REQUIRE(lda % 16 == 0 && ldb % 16 == 0 && lda >= (size_t)k && ldb >= (size_t)k, what);
+    EB_REQUIRE(lda < ((size_t)1 << 40) && ldb < ((size_t)1 << 40), what);
+    EB_REQUIRE(!m || !n || c, what);
+    EB_REQUIRE(!m || !n || !k || (qa && qb && scale_a && scale_b && aligned16(qa) && aligned16(qb)), what);
+    if (k > 0x7fffff00) return set_error(EDDLB200_ELIMIT, "%s: k = %d", what, k);
+    const size_t out = (size_t)m * n * sizeof(float);
+    const void *in[] = {qa, qb, scale_a, scale_b};
+    const size_t bytes[] = {matrix_bytes(m, k, lda), matrix_bytes(n, k, ldb), scale_bytes(m, k, block_a), scale_bytes(n, k, block_b)};
+    for (int i = 0; i < 4; i++) EB_REQUIRE(!overlap(c, out, in[i], bytes[i]), what);
+    EB_CTX(dev);
+    if (!m || !n) return 0;
+    for (int i = 0; i < 4; i++) EB_READS(in[i], bytes[i]);
+    if (!inc_c) EB_WRITES(c, out);
+    else {
+        EB_SETTLE(c, out);
+        int status = 0;
+        if (lz_take(cx, st, c, out, &status)) inc_c = 0;               // zeros owed to all of C: nothing to add to
+        if (status) return status;
+    }
+    ProfScope prof(cx, PROF_GEMM, 2.0 * m * n * k);
+    if (!k) return inc_c ? 0 : launch_zero_fill(cx, st, c, (size_t)m * n);
+    const int bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
+    const size_t tiles_p = ceil_div(n, 128), tiles = tiles_p * ceil_div(m, bn);
+    if (tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
+    ProdParams P;
+    if (!encode_bytes_map(&P.map_p, qb, ldb, n, k, 128) || !encode_bytes_map(&P.map_q, qa, lda, m, k, bn)) return set_error(EDDLB200_EINVAL, "%s: the driver refuses a tensor map of the operands", what);
+    P.scale_p = scale_b; P.scale_q = scale_a; P.c = c;
+    P.p_rows = n; P.q_rows = m; P.kblocks = (int)ceil_div(k, kBlk);
+    P.p_shift = block_b == kBlk ? 7 : 0; P.q_shift = block_a == kBlk ? 7 : 0;
+    P.p_scales = (int)ceil_div(n, block_b); P.q_scales = (int)ceil_div(m, block_a);
+    P.tiles_p = (int)tiles_p; P.inc = inc_c != 0;
+    size_t splits = EDDLB200_NUM_SMS / tiles;
+    if (splits > 8) splits = 8;
+    if (splits > (size_t)P.kblocks) splits = P.kblocks;
+    P.splits = (int)(splits < 1 ? 1 : splits);
+    P.idesc = fp8_idesc(format_b, format_a, 128, bn);
+    switch (bn) {
+        case 16: return launch_product<16>(cx, dev, st, P, (unsigned)tiles);
+        case 32: return launch_product<32>(cx, dev, st, P, (unsigned)tiles);
+        case 64: return launch_product<64>(cx, dev, st, P, (unsigned)tiles);
+        case 128: return launch_product<128>(cx, dev, st, P, (unsigned)tiles);
+        default: return launch_product<256>(cx, dev, st, P, (unsigned)tiles);
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,536 @@
+// What stands between two blocks of a residual net, as one pass: normalise the block's output, scale it by a gate, add it to the
+// scaled residual stream, normalise the sum for the next block -- and the backward pass of all of it.
+//
+//     z = norm(f) g1 + b1        r_out = s r + gate z        h = norm(r_out) g2 + b2
+//     norm(x) = (x - mean) / sqrt(mean((x - mean)^2) + eps) over a row; the RMS form leaves the mean out
+//
+// Both passes are bound by memory: 16 bytes a value forward (f, r read, r_out, h written), 24 backward (dh, dr_out, f, r_out read,
+// df, dr written).  A row is held in the registers of a team of threads, statistics are two-pass in fp32.
+#include <cooperative_groups.h>
+#include "common.cuh"
+
+namespace {
+
+using namespace eb;
+namespace cg = cooperative_groups;
+
+constexpr int kMaxCols = 16384;            // 1024 threads with four 16-byte pieces each; four blocks of 512 with two each
+
+// Sums of K values over a team of TPR threads (a warp, or the whole block); every thread gets them.  Two buffers take turns, so one
+// barrier is enough: a buffer is written again only after the barrier of the sums in between, which every reader has passed.
+template <int TPR, int K>
+struct TeamSum {
+    static constexpr int W = TPR / 32;
+    float *buf;
+    int flip = 0;
+    __device__ __forceinline__ TeamSum(float *b) : buf(b) {}
+    __device__ __forceinline__ void operator()(float (&v)[K]) {
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] = warp_sum(v[k]);
+        if (TPR == 32) return;
+        float *b = buf + flip * (K * W);
+        flip ^= 1;
+        const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+        if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < K; k++) b[k * W + w] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] = warp_sum(lane < W ? b[k * W + lane] : 0.f);
+    }
+};
+
+// The NV x 4 values that thread t of a team holds of a row: pieces of 16 bytes where VEC, single values a team apart otherwise.
+template <int TPR, int NV, bool VEC>
+struct Piece {
+    int t, cols;
+    __device__ __forceinline__ int at(int i) const { return VEC ? ((i / 4) * TPR + t) * 4 + i % 4 : i * TPR + t; }
+    __device__ __forceinline__ bool has(int i) const { return at(VEC ? i & ~3 : i) < cols; }
+    __device__ __forceinline__ void load(float (&v)[NV * 4], const float *p, float missing) const {
+        if (VEC) {
+#pragma unroll
+            for (int i = 0; i < NV * 4; i += 4) {
+                float4 q = make_float4(missing, missing, missing, missing);
+                if (p && has(i)) q = *reinterpret_cast<const float4 *>(p + at(i));
+                v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV * 4; i++) v[i] = p && has(i) ? p[at(i)] : missing;
+        }
+    }
+    __device__ __forceinline__ void store(float *p, const float (&v)[NV * 4]) const {
+        if (VEC) {
+#pragma unroll
+            for (int i = 0; i < NV * 4; i += 4)
+                if (has(i)) *reinterpret_cast<float4 *>(p + at(i)) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV * 4; i++) if (has(i)) p[at(i)] = v[i];
+        }
+    }
+};
+
+struct FwdArgs {
+    const float *f, *r, *gate, *g1, *b1, *g2, *b2;
+    float *r_out, *h, *stats;
+    float res_scale, eps;
+    int cols, rows, layer, post;            // rows: of one group
+    size_t total;
+};
+
+template <int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_fwd_kernel(const FwdArgs a) {
+    EB_GRID_WAIT();
+    __shared__ float sums[2 * (TPR / 32)];
+    TeamSum<TPR, 1> sum(sums);
+    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4;
+    const Piece<TPR, NV, VEC> piece{(int)(threadIdx.x % TPR), a.cols};
+    const float inv = 1.f / (float)a.cols;
+    // mean and 1 / deviation of the team's row; the values are centred in place
+    auto normalise = [&](float (&v)[N], float &mean, float &rstd) {
+        float s[1] = {0.f};
+        mean = 0.f;
+        if (a.layer) {
+#pragma unroll
+            for (int i = 0; i < N; i++) s[0] += v[i];                   // absent values are zero
+            sum(s);
+            mean = s[0] * inv;
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = piece.has(i) ? v[i] - mean : 0.f;
+        }
+        s[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) s[0] += v[i] * v[i];
+        sum(s);
+        rstd = __frcp_rn(sqrtf(s[0] * inv + a.eps));
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] *= rstd;
+    };
+    for (size_t row = (size_t)blockIdx.x * TEAMS + threadIdx.x / TPR; row < a.total; row += (size_t)gridDim.x * TEAMS) {
+        float v[N], x[N];
+        float mean1 = 0.f, rstd1 = 0.f, mean2 = 0.f, rstd2 = 0.f;
+        const size_t base = row * a.cols;
+        piece.load(x, a.r + base, 0.f);
+        if (a.f) {
+            piece.load(v, a.f + base, 0.f);
+            if (a.post) normalise(v, mean1, rstd1);
+            float p[N];
+            if (a.g1) {
+                piece.load(p, a.g1, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[i] *= p[i];
+            }
+            if (a.b1) {
+                piece.load(p, a.b1, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[i] += p[i];
+            }
+            if (a.gate) {
+                piece.load(p, a.gate + row / a.rows * a.cols, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[i] *= p[i];
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] = a.res_scale * x[i] + v[i];
+            piece.store(a.r_out + base, x);
+        }
+        if (a.h) {
+            normalise(x, mean2, rstd2);
+            float p[N];
+            if (a.g2) {
+                piece.load(p, a.g2, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] *= p[i];
+            }
+            if (a.b2) {
+                piece.load(p, a.b2, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] += p[i];
+            }
+            piece.store(a.h + base, x);
+        }
+        if (a.stats && piece.t == 0) *reinterpret_cast<float4 *>(a.stats + row * 4) = make_float4(mean1, rstd1, mean2, rstd2);
+    }
+}
+
+struct BwdArgs {
+    const float *dh, *dr_out, *f, *r_out, *gate, *g1, *b1, *g2, *stats;
+    float *df, *dr;
+    float *param_part, *gate_part;          // [block][4][cols] of dg2, db2, dg1, db1; [unit][cols] of dgate, which is dgate itself where a unit is a group
+    float res_scale;
+    int cols, rows, layer, post, inc_df, inc_dr;         // inc: 0 store, 1 add, 2 add to a destination known to hold zeros
+    int want_gate, want_param, inc_gate;    // want_param: bits dg2, db2, dg1, db1; inc_gate: add to gate_part
+    int unit_groups, slices, workers;       // a unit is a slice of a group's rows; workers: blocks (clusters) that share the units
+    size_t unit_rows;                       // rows of one unit group
+};
+
+// Backward.  With n1, n2 the normalised rows, dn2 = dh g2, G = gate g1 and <> the mean over a row:
+//     u  = dr_out + rstd2 (dn2 - <dn2> - n2 <dn2 n2>)                      (the gradient of r_out; RMS: without <dn2>)
+//     dr = s u,   dn1 = G u,   df = rstd1 (dn1 - <dn1> - n1 <dn1 n1>)
+//     dg2 = sum dh n2, db2 = sum dh, dg1 = sum gate u n1, db1 = sum gate u over all rows, dgate = sum u z over a group's
+// u is linear in <dn2> and <dn2 n2>, so the sums of the second norm follow from sums of known values:
+//     <dn1>    = <G e> - rstd2 (<dn2> <G>    + <dn2 n2> <G n2>),       e = dr_out + rstd2 dn2
+//     <dn1 n1> = <G e n1> - rstd2 (<dn2> <G n1> + <dn2 n2> <G n2 n1>)
+// and a row takes one exchange between its threads instead of two.  The column sums stay in registers over all rows of a block
+// and are added in a fixed order afterwards: no atomics.
+template <int TPR, int NV, bool VEC, bool GENERAL, bool CLUSTER>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kernel(const BwdArgs a) {
+    EB_GRID_WAIT();
+    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4, K = GENERAL ? 8 : 3;
+    extern __shared__ float team_sums[];                               // TPR == 32: the column sums of the block's teams, one kind at a time
+    __shared__ float sums[2 * K * (TPR / 32)];
+    __shared__ float peers[CLUSTER ? 2 * K * 4 : 1];
+    TeamSum<TPR, K> sum(sums);
+    const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0, csize = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
+    const int worker = (int)(blockIdx.x / csize), col0 = rank * (TPR * N), cols_here = min(a.cols - col0, TPR * N);
+    const Piece<TPR, NV, VEC> piece{(int)(threadIdx.x % TPR), cols_here};
+    const int team = threadIdx.x / TPR;
+    const float inv = 1.f / (float)a.cols;
+    int flip = 0;
+    float g2[N], gg[N], acc[GENERAL ? 4 : 2][N] = {}, acc_gate[N] = {};
+    piece.load(g2, a.g2 ? a.g2 + col0 : nullptr, a.g2 ? 0.f : 1.f);
+    if (!a.dh) {
+#pragma unroll
+        for (int i = 0; i < N; i++) g2[i] = 0.f;
+    }
+    const int units = a.unit_groups * a.slices;
+    for (int unit = worker; unit < units; unit += a.workers) {
+        const size_t group = unit / a.slices, slice = unit % a.slices;
+        const size_t first = group * a.unit_rows + a.unit_rows * slice / a.slices, last = group * a.unit_rows + a.unit_rows * (slice + 1) / a.slices;
+        for (size_t row = first + team; row < last; row += TEAMS) {
+            const size_t base = row * a.cols + col0;
+            const float4 st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
+            float dh[N], e[N], n1[N], n2[N], gate[N];
+            piece.load(dh, a.dh ? a.dh + base : nullptr, 0.f);
+            piece.load(e, a.dr_out ? a.dr_out + base : nullptr, 0.f);
+            piece.load(n2, a.dh ? a.r_out + base : nullptr, 0.f);
+            piece.load(n1, a.f ? a.f + base : nullptr, 0.f);
+            piece.load(gate, a.gate ? a.gate + row / a.rows * a.cols + col0 : nullptr, 1.f);
+            if (a.g1) {
+                piece.load(gg, a.g1 + col0, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) gg[i] *= gate[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) gg[i] = gate[i];
+            }
+            float s[K] = {};
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (!piece.has(i)) { n1[i] = n2[i] = 0.f; gg[i] = 0.f; continue; }
+                n2[i] = (n2[i] - st.z) * st.w;
+                if (a.post) n1[i] = (n1[i] - st.x) * st.y;
+                const float dn2 = dh[i] * g2[i];
+                e[i] += st.w * dn2;
+                s[0] += dn2 * n2[i];
+                s[1] += gg[i] * e[i] * n1[i];
+                s[2] += gg[i] * n2[i] * n1[i];
+                if (GENERAL) {
+                    s[3] += dn2;
+                    s[4] += gg[i] * e[i];
+                    s[5] += gg[i];
+                    s[6] += gg[i] * n2[i];
+                    s[7] += gg[i] * n1[i];
+                }
+            }
+            sum(s);
+            if (CLUSTER) {
+                cg::cluster_group cl = cg::this_cluster();
+                float *mine = peers + flip * (K * 4);
+                flip ^= 1;
+                if (threadIdx.x < (unsigned)csize) {
+                    float *there = cl.map_shared_rank(mine, threadIdx.x);
+#pragma unroll
+                    for (int k = 0; k < K; k++) there[k * 4 + rank] = s[k];
+                }
+                cl.sync();
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    s[k] = 0.f;
+                    for (int c = 0; c < csize; c++) s[k] += mine[k * 4 + c];
+                }
+            }
+            const float m_n2 = s[0] * inv, m_1 = GENERAL && a.layer ? s[3] * inv : 0.f;
+            const float q_n1 = s[1] * inv - st.w * (m_n2 * (s[2] * inv) + (GENERAL ? m_1 * (s[7] * inv) : 0.f));
+            const float q_1 = GENERAL && a.layer ? s[4] * inv - st.w * (m_n2 * (s[6] * inv) + m_1 * (s[5] * inv)) : 0.f;
+            float out[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float u = e[i] - st.w * (m_1 + n2[i] * m_n2);
+                acc[0][i] += dh[i] * n2[i];
+                acc[1][i] += gate[i] * u * n1[i];
+                if (GENERAL) { acc[2][i] += dh[i]; acc[3][i] += gate[i] * u; }
+                e[i] = u;
+                const float dn1 = gg[i] * u;
+                out[i] = a.post ? st.y * (dn1 - q_1 - n1[i] * q_n1) : dn1;
+            }
+            if (a.df) {
+                if (a.inc_df) {
+                    float old[N];
+                    piece.load(old, a.inc_df == 1 ? a.df + base : nullptr, 0.f);
+#pragma unroll
+                    for (int i = 0; i < N; i++) out[i] += old[i];
+                }
+                piece.store(a.df + base, out);
+            }
+            if (a.want_gate) {
+                float p[N], b[N];
+                piece.load(p, a.g1 ? a.g1 + col0 : nullptr, 1.f);
+                piece.load(b, a.b1 ? a.b1 + col0 : nullptr, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) acc_gate[i] += e[i] * (n1[i] * p[i] + b[i]);
+            }
+            if (a.dr) {
+                if (a.inc_dr) {
+                    piece.load(out, a.inc_dr == 1 ? a.dr + base : nullptr, 0.f);
+#pragma unroll
+                    for (int i = 0; i < N; i++) out[i] += a.res_scale * e[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; i++) out[i] = a.res_scale * e[i];
+                }
+                piece.store(a.dr + base, out);
+            }
+        }
+        if (a.want_gate) {
+            float *dst = a.gate_part + (size_t)unit * a.cols + col0;
+            if (TEAMS == 1) {
+                if (a.inc_gate) {
+                    float old[N];
+                    piece.load(old, dst, 0.f);
+#pragma unroll
+                    for (int i = 0; i < N; i++) acc_gate[i] += old[i];
+                }
+                piece.store(dst, acc_gate);
+            } else {
+                __syncthreads();
+                piece.store(team_sums + team * a.cols, acc_gate);
+                __syncthreads();
+                for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+                    float t = 0.f;
+                    for (int k = 0; k < TEAMS; k++) t += team_sums[k * a.cols + c];
+                    dst[c] = a.inc_gate ? dst[c] + t : t;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++) acc_gate[i] = 0.f;
+        }
+    }
+    // kinds in the order of param_part: dg2, db2, dg1, db1
+#pragma unroll
+    for (int kind = 0; kind < 4; kind++) {
+        if (!(a.want_param >> kind & 1)) continue;
+        const int which = kind == 0 ? 0 : kind == 1 ? 2 : kind == 2 ? 1 : 3;
+        if (!GENERAL && which >= 2) continue;
+        float *dst = a.param_part + ((size_t)worker * 4 + kind) * a.cols + col0;
+        if (TEAMS == 1) piece.store(dst, acc[GENERAL ? which : which & 1]);
+        else {
+            __syncthreads();
+            piece.store(team_sums + team * a.cols, acc[GENERAL ? which : which & 1]);
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+                float t = 0.f;
+                for (int k = 0; k < TEAMS; k++) t += team_sums[k * a.cols + c];
+                dst[c] = t;
+            }
+        }
+    }
+    if (CLUSTER) cg::this_cluster().sync();                 // a block's slots outlive the writes of the others
+}
+
+// Column sums of the partial rows, in a fixed order: y 0..3 the parameters' gradients, from 4 on dgate of group y - 4.
+struct FoldArgs {
+    const float *param_part, *gate_part;
+    float *out[4], *dgate;
+    int cols, workers, slices, inc;
+};
+constexpr int kFoldRows = 16;
+__global__ void __launch_bounds__(32 * kFoldRows) norm_residual_fold_kernel(const FoldArgs a) {
+    EB_GRID_WAIT();
+    __shared__ float part[kFoldRows][33];
+    const int col = blockIdx.x * 32 + threadIdx.x;
+    const bool gate = blockIdx.y >= 4;
+    float *out = gate ? a.dgate + (size_t)(blockIdx.y - 4) * a.cols : a.out[blockIdx.y & 3];
+    if (!gate && !out) return;
+    const float *src = gate ? a.gate_part + (size_t)(blockIdx.y - 4) * a.slices * a.cols : a.param_part + (size_t)blockIdx.y * a.cols;
+    const size_t step = gate ? a.cols : (size_t)4 * a.cols;
+    const int n = gate ? a.slices : a.workers;
+    float s = 0.f;
+    if (col < a.cols) {
+#pragma unroll 4
+        for (int i = threadIdx.y; i < n; i += kFoldRows) s += __ldcg(src + i * step + col);
+    }
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y || col >= a.cols) return;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < kFoldRows; i++) t += part[i][threadIdx.x];
+    out[col] = a.inc ? out[col] + t : t;
+}
+
+template <int TPR, int NV>
+void launch_fwd(cudaStream_t st, const FwdArgs &a, bool vec) {
+    constexpr int block = TPR == 32 ? 256 : TPR, teams = TPR == 32 ? 8 : 1;
+    const size_t want = ceil_div(a.total, teams), most = (size_t)EDDLB200_NUM_SMS * (2048 / block);
+    const unsigned grid = (unsigned)(want < most ? want : most);
+    eb::launch(vec ? norm_residual_fwd_kernel<TPR, NV, true> : norm_residual_fwd_kernel<TPR, NV, false>, grid, block, 0, st, a);
+}
+
+template <int TPR, int NV, bool CLUSTER>
+void launch_bwd(cudaStream_t st, const BwdArgs &a, bool vec, bool general, unsigned csize) {
+    constexpr int block = TPR == 32 ? 256 : TPR;
+    const size_t smem = TPR == 32 ? (size_t)8 * a.cols * sizeof(float) : 0;
+    auto kernel = vec ? (general ? norm_residual_bwd_kernel<TPR, NV, true, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, true, false, CLUSTER>)
+                      : (general ? norm_residual_bwd_kernel<TPR, NV, false, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, false, false, CLUSTER>);
+    if (CLUSTER) eb::launch_cluster(kernel, csize, a.workers * csize, block, smem, st, a);
+    else eb::launch(kernel, a.workers, block, smem, st, a);
+}
+
+// An output may be an input's own memory (every value is read before it is written, by the thread that writes it), but not part of it.
+bool clash(const void *out, size_t out_bytes, const void *in, size_t in_bytes) { return out != in && overlap(out, out_bytes, in, in_bytes); }
+
+const char *const kFwd = "norm_residual_fwd", *const kBwd = "norm_residual_bwd";
+
+}  // namespace
+
+using namespace eb;
+
+extern "C" {
+
+int eddlb200_norm_residual_fwd(int dev, int kind, int post, int groups, int rows, int cols, const float *f, const float *r, const float *gate,
+                               const float *g1, const float *b1, float res_scale, const float *g2, const float *b2, float eps,
+                               float *r_out, float *h, float *stats) {
+    EB_REQUIRE((kind == 0 || kind == 1) && (post == 0 || post == 1), kFwd);
+    EB_REQUIRE(groups >= 0 && rows >= 0 && cols > 0, kFwd);
+    EB_REQUIRE(eps >= 0.f, kFwd);
+    if (cols > kMaxCols) return set_error(EDDLB200_ELIMIT, "%s: rows of %d values, at most %d", kFwd, cols, kMaxCols);
+    EB_REQUIRE((f != nullptr) == (r_out != nullptr), kFwd);
+    EB_REQUIRE(f || (!gate && !g1 && !b1 && !post && res_scale == 1.f), kFwd);
+    EB_REQUIRE(post || (!g1 && !b1), kFwd);
+    EB_REQUIRE(h || (f && !g2 && !b2), kFwd);
+    EB_REQUIRE(aligned16(stats), kFwd);
+    const size_t total = (size_t)groups * rows, bytes = total * cols * sizeof(float), vector = (size_t)cols * sizeof(float), gates = groups * vector;
+    EB_REQUIRE(!total || r, kFwd);
+    const void *in[] = {f, r, gate, g1, b1, g2, b2};
+    const size_t in_bytes[] = {bytes, bytes, gates, vector, vector, vector, vector};
+    for (int i = 0; i < 7; i++) {
+        EB_REQUIRE(i < 2 ? !clash(r_out, bytes, in[i], in_bytes[i]) : !overlap(r_out, bytes, in[i], in_bytes[i]), kFwd);
+        EB_REQUIRE(i < 2 ? !clash(h, bytes, in[i], in_bytes[i]) : !overlap(h, bytes, in[i], in_bytes[i]), kFwd);
+        EB_REQUIRE(!overlap(stats, total * 16, in[i], in_bytes[i]), kFwd);
+    }
+    EB_REQUIRE(!overlap(r_out, bytes, h, bytes) && !overlap(stats, total * 16, r_out, bytes) && !overlap(stats, total * 16, h, bytes), kFwd);
+    EB_CTX(dev);
+    if (!total) return 0;
+    for (int i = 0; i < 7; i++) EB_READS(in[i], in_bytes[i]);
+    EB_WRITES(r_out, bytes); EB_WRITES(h, bytes); EB_WRITES(stats, total * 16);
+    ProfScope prof(cx, PROF_BN_FWD, (double)bytes * ((f ? 3 : 1) + (h ? 1 : 0)));
+    const FwdArgs a{f, r, gate, g1, b1, g2, b2, r_out, h, stats, res_scale, eps, cols, rows, kind, post, total};
+    const bool vec = cols % 4 == 0 && aligned16(f) && aligned16(r) && aligned16(gate) && aligned16(g1) && aligned16(b1) && aligned16(g2) && aligned16(b2) && aligned16(r_out) && aligned16(h);
+    if (cols <= 128) launch_fwd<32, 1>(st, a, vec);
+    else if (cols <= 256) launch_fwd<32, 2>(st, a, vec);
+    else if (cols <= 512) launch_fwd<128, 1>(st, a, vec);
+    else if (cols <= 1024) launch_fwd<128, 2>(st, a, vec);
+    else if (cols <= 2048) launch_fwd<256, 2>(st, a, vec);
+    else if (cols <= 4096) launch_fwd<512, 2>(st, a, vec);
+    else if (cols <= 8192) launch_fwd<1024, 2>(st, a, vec);
+    else launch_fwd<1024, 4>(st, a, vec);
+    EB_LAUNCH_CHECK(kFwd);
+    return 0;
+}
+
+int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows, int cols, const float *dh, const float *dr_out, const float *f,
+                               const float *r_out, const float *gate, const float *g1, const float *b1, float res_scale, const float *g2,
+                               const float *stats, float *df, float *dr, int inc_d, float *dgate, float *dg1, float *db1, float *dg2, float *db2, int inc_g) {
+    EB_REQUIRE((kind == 0 || kind == 1) && (post == 0 || post == 1), kBwd);
+    EB_REQUIRE(groups >= 0 && rows >= 0 && cols > 0, kBwd);
+    if (cols > kMaxCols) return set_error(EDDLB200_ELIMIT, "%s: rows of %d values, at most %d", kBwd, cols, kMaxCols);
+    EB_REQUIRE(dh || dr_out, kBwd);
+    EB_REQUIRE(dh || (!g2 && !dg2 && !db2), kBwd);
+    EB_REQUIRE(f || (!gate && !g1 && !b1 && !post && res_scale == 1.f && !df), kBwd);
+    EB_REQUIRE(f || !(dgate || dg1 || db1), kBwd);
+    EB_REQUIRE(post || (!g1 && !b1 && !dg1 && !db1), kBwd);
+    EB_REQUIRE(gate || !dgate, kBwd);
+    const size_t total = (size_t)groups * rows, bytes = total * cols * sizeof(float), vector = (size_t)cols * sizeof(float), gates = groups * vector;
+    EB_REQUIRE(!total || (stats && aligned16(stats) && (r_out || !dh)), kBwd);
+    const void *in[] = {dh, dr_out, f, r_out, gate, g1, b1, g2, stats};
+    const size_t in_bytes[] = {bytes, bytes, bytes, bytes, gates, vector, vector, vector, total * 16};
+    float *out[] = {df, dr, dgate, dg1, db1, dg2, db2};
+    const size_t out_bytes[] = {bytes, bytes, gates, vector, vector, vector, vector};
+    for (int o = 0; o < 7; o++) {
+        for (int i = 0; i < 9; i++) EB_REQUIRE(o < 2 && i < 4 ? !clash(out[o], out_bytes[o], in[i], in_bytes[i]) : !overlap(out[o], out_bytes[o], in[i], in_bytes[i]), kBwd);
+        for (int q = 0; q < o; q++) EB_REQUIRE(!overlap(out[o], out_bytes[o], out[q], out_bytes[q]), kBwd);
+        EB_REQUIRE(!(o < 2 && inc_d && out[o]) || (out[o] != dh && out[o] != dr_out && out[o] != f && out[o] != r_out), kBwd);
+    }
+    EB_CTX(dev);
+    const bool cluster = cols > 4096;
+    const unsigned csize = cluster ? (unsigned)ceil_div(cols, 4096) : 1;
+    const int team_rows = cols <= 256 ? 8 : 1, block = cols <= 256 ? 256 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : 512;
+    BwdArgs a{dh, dr_out, f, r_out, gate, g1, b1, g2, stats, df, dr, nullptr, nullptr, res_scale, cols, rows, kind, post, 0, 0};
+    a.want_gate = dgate != nullptr;
+    a.want_param = (dg2 ? 1 : 0) | (db2 ? 2 : 0) | (dg1 ? 4 : 0) | (db1 ? 8 : 0);
+    a.unit_groups = dgate ? groups : 1;
+    a.unit_rows = dgate ? (size_t)rows : total;
+    const size_t most = (size_t)EDDLB200_NUM_SMS * (1024 / block) / csize, passes = total ? ceil_div(a.unit_rows, team_rows) : 1;
+    size_t slices = a.unit_groups ? ceil_div(most, a.unit_groups) : 1;
+    if (slices > passes) slices = passes;
+    if (slices < 1) slices = 1;
+    const size_t units = a.unit_groups * slices;
+    a.slices = (int)slices;
+    a.workers = (int)(units < most ? units : most);
+    const size_t param_floats = a.want_param ? (size_t)a.workers * 4 * cols : 0, gate_floats = dgate && slices > 1 ? units * cols : 0;
+    const bool fold = a.want_param || gate_floats;
+    a.gate_part = dgate;
+    a.inc_gate = dgate && !gate_floats && inc_g;
+    if (total && fold) {
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        if (int e = cuda_status(cudaStreamIsCapturing(st, &capturing), kBwd)) return e;
+        if (capturing != cudaStreamCaptureStatusNone) return set_error(EDDLB200_EINVAL, "%s: the column sums use the library's scratch memory, which a captured graph must not hold", kBwd);
+        float *scr = (float *)scratch(cx, (param_floats + gate_floats) * sizeof(float));
+        if (!scr) return cudaErrorMemoryAllocation;
+        a.param_part = scr;
+        if (gate_floats) a.gate_part = scr + param_floats;
+    }
+    if (total) for (int i = 0; i < 9; i++) EB_READS(in[i], in_bytes[i]);
+    int inc[2] = {inc_d != 0, inc_d != 0};
+    for (int o = 0; o < 7; o++) {
+        if (!out[o]) continue;
+        if (o < 2 ? !inc_d : !inc_g) EB_WRITES(out[o], out_bytes[o]);
+        else if (o >= 2) EB_MODIFIES(out[o], out_bytes[o]);
+        else {
+            EB_SETTLE(out[o], out_bytes[o]);
+            int status = 0;
+            if (lz_take(cx, st, out[o], out_bytes[o], &status)) inc[o] = 2;      // zeros owed to all of it: nothing to read
+            if (status) return status;
+        }
+    }
+    a.inc_df = inc[0]; a.inc_dr = inc[1];
+    if (!total) {                            // the sums over no rows are zero
+        for (int o = 2; o < 7 && !inc_g; o++)
+            if (out[o] && out_bytes[o]) if (int e = launch_zero_fill(cx, st, out[o], out_bytes[o] / sizeof(float))) return e;
+        return 0;
+    }
+    ProfScope prof(cx, PROF_BN_BWD, (double)bytes * ((dh ? 2 : 0) + (dr_out ? 1 : 0) + (f ? 1 : 0) + (df ? 1 + (inc[0] == 1) : 0) + (dr ? 1 + (inc[1] == 1) : 0)));
+    const bool general = kind || db1 || db2;
+    bool vec = cols % 4 == 0;
+    for (int i = 0; i < 8; i++) vec = vec && aligned16(in[i]);
+    vec = vec && aligned16(df) && aligned16(dr);
+    if (cols <= 128) launch_bwd<32, 1, false>(st, a, vec, general, 1);
+    else if (cols <= 256) launch_bwd<32, 2, false>(st, a, vec, general, 1);
+    else if (cols <= 512) launch_bwd<128, 1, false>(st, a, vec, general, 1);
+    else if (cols <= 1024) launch_bwd<128, 2, false>(st, a, vec, general, 1);
+    else if (cols <= 2048) launch_bwd<256, 2, false>(st, a, vec, general, 1);
+    else if (cols <= 4096) launch_bwd<512, 2, false>(st, a, vec, general, 1);
+    else launch_bwd<512, 2, true>(st, a, vec, general, csize);
+    EB_LAUNCH_CHECK(kBwd);
+    if (!fold) return 0;
+    const FoldArgs fa{a.param_part, a.gate_part, {dg2, db2, dg1, db1}, dgate, cols, a.workers, a.slices, inc_g};
+    const unsigned kinds = 4 + (gate_floats ? (unsigned)groups : 0);           // fewer groups than units that run at a time, so far below the grid's limit
+    eb::launch(norm_residual_fold_kernel, dim3((unsigned)ceil_div(cols, 32), kinds), dim3(32, kFoldRows), 0, st, fa);
+    EB_LAUNCH_CHECK(kBwd);
+    return 0;
+}
+
+}  // extern "C"

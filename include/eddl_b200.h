@@ -128,6 +128,20 @@ int eddlb200_cce_delta(int dev, const float *y_true, const float *y_pred, float 
 /* rows whose argmax(y_true) == argmax(y_pred), first maximum wins.  Blocking unless remembered (see above). */
 int eddlb200_accuracy(int dev, const float *y_true, const float *y_pred, int rows, int cols, int *host_out);
 
+/* Distillation (no counterpart in EDDL): loss of a student's logits [rows, cols] (rows `ld` floats apart, like delta's; at most 401408 columns)
+ * against the teacher's k <= 1024 best classes of each row -- ids [rows, k] and teacher [rows, k], the teacher's logits -- mixed with the
+ * cross-entropy of hard labels [rows], and its gradient.  With x a row, q = softmax(x / T), T = temperature:
+ *   loss[row] = w ((1 - alpha) T^2 KL + alpha (log sum exp x - x_label)),   delta = d loss[row] / d x
+ *   teacher_lse null:  KL = sum_j p_j log(p_j / q_j),  p = softmax of teacher / T over the row's entries
+ *   else [rows], log sum exp(t / T) over ALL of the teacher's classes:  p_j = exp(teacher_j / T - teacher_lse), and p_r = max(0, 1 - sum p_j), the
+ *          rest, is one class more: KL += p_r log(p_r / q_r), q_r the student's mass outside the entries
+ * w = weights[row] (null: 1).  An id outside 0 .. cols - 1 is padding, of a repeated id the first entry counts; a label outside 0 .. cols - 1 has
+ * no cross-entropy; a row of weight 0, or whose logits are all -infinity, has loss and delta 0 and nothing of a weightless row is read.  Logits of
+ * -infinity are classes that are masked out.  labels may be null when alpha is 0; delta may be null, or logits itself.  delta's columns
+ * from cols to ld keep what they hold. */
+int eddlb200_distill(int dev, const float *logits, const int *ids, const float *teacher, const float *teacher_lse, const int *labels,
+                     const float *weights, int rows, int cols, size_t ld, int k, float temperature, float alpha, float *loss, float *delta);
+
 /* ---- batch normalisation (src/hardware/gpu/nn/gpu_bn.cu:65-117;
  *      src/hardware/cpu/nn/cpu_bn.cpp:118-249).  x is [b, z, rc].  Argument order and
  *      meaning are those of gpu_batchnorm_forward / gpu_batchnorm_backward:
@@ -171,6 +185,26 @@ int eddlb200_bn_bwd(int dev, int b, int z, int rc,
                     float *delta, const float *opa, float *pdelta,
                     float *gbn_g, float *gbn_b, const float *bn_g,
                     const float *variance, float *mean1, float *mean2);
+
+/* ---- norms before and after a block, with its gate and the scale of the residual stream (no counterpart in EDDL, whose LAdd and
+ *      normalisation layers are separate).  Tensors are [groups * rows, cols], at most 16384 columns; gate is [groups, cols] and
+ *      applies to its group's rows (one group: a gate for each channel; groups of one row: one for each value); the other vectors are [cols].
+ *        z = (post ? norm(f) : f) * g1 + b1       r_out = res_scale * r + gate * z       h = norm(r_out) * g2 + b2
+ *      norm over a row: kind 0 x / sqrt(mean(x^2) + eps), kind 1 (x - mean) / sqrt(mean((x - mean)^2) + eps).
+ *      null: gate, g1, g2 = 1, b1, b2 = 0 (g1, b1 need post);  h = not wanted;  f = no block yet: h = norm(r) alone, and gate, g1, b1, r_out
+ *      are null, post 0, res_scale 1.  stats (16-byte aligned, [groups * rows, 4]: mean and 1/deviation of both norms) is what the backward pass needs; null
+ *      when there is none.  r_out may be r or f itself, h may be r or f itself. */
+int eddlb200_norm_residual_fwd(int dev, int kind, int post, int groups, int rows, int cols,
+                               const float *f, const float *r, const float *gate, const float *g1, const float *b1, float res_scale,
+                               const float *g2, const float *b2, float eps, float *r_out, float *h, float *stats);
+/* Gradients of sum(dh * h) + sum(dr_out * r_out) with respect to f, r, gate, g1, b1, g2, b2: stored, or with inc_d (df, dr) / inc_g
+ * (the others) added to what is there.  dh or dr_out may be null (a last or first norm of a net); any result may be.  r_out: as the forward pass
+ * wrote it (r where there was no f); stats: of that pass.  df and dr may be dh, dr_out, f or r_out itself unless inc_d.  Sums over rows are added
+ * in a fixed order in the library's scratch memory, so a call with any of dgate .. db2 is refused while the stream is captured. */
+int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows, int cols,
+                               const float *dh, const float *dr_out, const float *f, const float *r_out,
+                               const float *gate, const float *g1, const float *b1, float res_scale, const float *g2, const float *stats,
+                               float *df, float *dr, int inc_d, float *dgate, float *dg1, float *db1, float *dg2, float *db2, int inc_g);
 
 /* ---- pooling (src/hardware/gpu/nn/gpu_pool.cu:26-60,101-135;
  *      src/hardware/cpu/nn/cpu_pool.cpp:74-145,226-304).  Input [n,c,ih,iw], output
@@ -240,6 +274,29 @@ int eddlb200_mult2d(int dev, const float *a, int ta, const float *b, int tb, flo
 int eddlb200_sum2d_rowwise(int dev, const float *a, const float *b, float *c, int rows, int cols); /* C = A + b[col] */
 /* gpu_reduce_sum2D: axis 0 -> B[cols] (+)= sum over rows; axis 1 -> B[rows] (+)= sum over cols */
 int eddlb200_reduce_sum2d(int dev, const float *a, float *b, int rows, int cols, int axis, int inc_b);
+
+/* ---- dense algebra in 8-bit floating point with an fp32 scale for each block of 128 values along the reduction (no counterpart in
+ *      EDDL; beside eddlb200_mult2d).  A matrix [r, c] in 8 bits is r rows of c bytes, `ld` bytes apart (ld >= c, a multiple of 16, the
+ *      matrix 16-byte aligned; bytes between rows are neither read as values nor written), and a scale array [ceil(c/128)][ceil(r/block_rows)]: scale
+ *      [b][i] belongs to columns 128 b .. 128 b + 127 of row i (block_rows = 1) or of rows 128 i .. 128 i + 127 (block_rows = 128).  Formats: */
+#define EDDLB200_E4M3 0         /* 4 exponent bits, 3 mantissa bits, largest 448 */
+#define EDDLB200_E5M2 1         /* 5 exponent bits, 2 mantissa bits, largest 57344 */
+/* q = a in 8 bits with its scales and / or qt = the transpose of a ([cols, rows], blocks of 128 along a's rows) with its own, in one pass
+ * over a [rows, cols]: what the forward product and the weight gradient of a dense layer need of the same tensor.  Either of q, qt may
+ * be null (with its scale).  With peak the largest magnitude of a block, at least 2^-100:
+ *   pow2 = 0: scale = peak / largest, value = round(a * (largest / peak))        (each operation rounded to fp32, then to nearest even)
+ *   pow2 = 1: scale = the least power of two >= peak / largest, value = round(a / scale): nothing but the 8 bits is rounded.
+ * A NaN becomes the format's NaN and its block is scaled by the others; an infinity makes its block's scale infinite and becomes a NaN, so
+ * that it is not lost silently: what the block takes part in is then not finite. */
+int eddlb200_fp8_quantize(int dev, const float *a, int rows, int cols, int format, int block_rows, int pow2,
+                          void *q, size_t ldq, float *scale, void *qt, size_t ldqt, float *scale_t);
+/* C[m,n] = (inc_c ? C : 0) + sum over blocks b of 128 columns: scale_a[b][row's block] * scale_b[b][row's block] * sum_{k in b} qa[m,k] qb[n,k].
+ * Both operands are stored with k along their rows.  A dense layer y = x w^T is this product of x and w; its input gradient that of dy
+ * and the transposed w; its weight gradient that of the transposed dy and the transposed x.  Products and sums of a block are those of
+ * the tensor cores with fp32 accumulators, blocks are scaled and added in fp32; the order is fixed.  block_a, block_b: 1 or 128 rows. */
+int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_a, int format_a, int block_a,
+                        const void *qb, size_t ldb, const float *scale_b, int format_b, int block_b,
+                        float *c, int inc_c, int m, int n, int k);
 
 /* ---- Conv2D (src/hardware/gpu/nn/gpu_conv.cu:159-372;
  *      src/hardware/cpu/nn/cpu_conv.cpp:114-280,316-527).  Cross-correlation, zero padding,
