@@ -8,8 +8,10 @@
 //     delta = w [ (1 - alpha) T ( q_i - p_i ) + alpha (softmax(x)_i - [i = label]) ],    q_i (1 - p_r / q_r) for i outside the entries
 //
 // Bound by memory: 8 bytes a logit.  A row lies in shared memory between its one read and its one write -- of one block, or in
-// pieces in the blocks of a cluster, which exchange two sets of sums (the maxima, then what depends on them).  Mass outside the
-// entries is summed from the values outside, not as 1 minus something: entries are replaced by -infinity first.
+// pieces in the blocks of a cluster.  What has to do with the entries (a few dozen a row: look-ups, repeated ids, 64-bit
+// exponentials) is a chain of latencies as long as the streaming of the row, so it has a warp of its own that works one row ahead; the
+// other warps keep a running maximum and sum a thread and meet once a row.  Mass outside the entries is summed from the
+// values outside, not as 1 minus something: with `teacher_lse` the entries' cells are set to -infinity before the sum.
 #include <type_traits>
 #include <cooperative_groups.h>
 #include "common.cuh"
@@ -20,16 +22,15 @@ using namespace eb;
 namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 1024;
-constexpr int kMaxPiece = 50176;                 // logits of a row in one block: 196 KB of shared memory, with 12 KB of entries
 constexpr int kMaxCluster = 8;
+constexpr int kMaxPiece = 43008;                 // logits of a row in one block: 168 KB of shared memory, with up to 44 KB of entries
 constexpr int kMaxCols = kMaxPiece * kMaxCluster;
-constexpr int kSums = 6;
 
 struct Args {
     const float *x, *teacher, *teacher_lse, *weights;
     const int *ids, *labels;
     float *loss, *delta;
-    int rows, cols, k, piece;                    // piece: logits of one block, a multiple of 4
+    int rows, cols, k, piece, slots;             // piece: logits of one block, a multiple of 4; slots: of the table of ids seen, a power of two
     size_t ld;
     float temperature, alpha;
 };
@@ -37,217 +38,421 @@ struct Args {
 __device__ __forceinline__ float minus_inf() { return __int_as_float(0xff800000); }
 // a NaN on either side stays
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
-__device__ __forceinline__ double max_nan(double a, double b) { return b > a || b != b ? b : a; }
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float exp2_fast(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+constexpr float kLog2e = 1.44269504f;
 
-// TEAM threads share a row (or a piece of it): a warp, or the whole block.  CLUSTER: the pieces of a row are the blocks of a cluster.
-template <int TEAM, bool VEC, bool CLUSTER>
-__global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM) distill_kernel(const Args a) {
-    constexpr int TEAMS = TEAM == 32 ? 8 : 1, W = TEAM / 32;
+// What a row's entries and its label add.  loss = base + per_z ((m - anchor) / T + ln z) - per_rest (ln z_out - ln z) + hard (m - x_label + ln z_1), with
+// m the row's largest logit, z and z_1 the sums of exp((x - m) / T) and exp(x - m), z_out the first one outside the entries; the gradient is
+// inside / z - rest / z_out times the exponential outside the entries, inside / z times it minus `less` at an entry.
+struct Head {
+    double base, per_z, per_rest, hard;
+    float inside, rest, x_label, anchor;         // anchor: the largest of the entries' logits
+    float z, z1;                                 // the entries' sums relative to it, where their cells are closed
+    int label, label_is_entry, live;
+};
+struct Record {
+    Head *head;
+    float *value, *less;                         // of an entry: the student's logit, what the teacher takes off its gradient
+    int *id;                                     // -1: padding, or an id that came before
+};
+
+// What the look-up of a row begins with, asked for while the row before is worked on: its numbers and its first entries.
+constexpr int kAhead = 4;                        // times 32 entries
+struct Ahead {
+    float weight = 1.f, lse = 0.f, t[kAhead];
+    int label = -1, id[kAhead];
+    __device__ __forceinline__ void ask(const Args &a, int row) {
+        if (row >= a.rows) return;
+        const int lane = threadIdx.x & 31;
+        if (a.weights) weight = a.weights[row];
+        if (a.teacher_lse) lse = a.teacher_lse[row];
+        if (a.alpha != 0.f) label = a.labels[row];
+        if (a.alpha != 1.f) entries(a, row, 0, lane);
+    }
+    __device__ __forceinline__ void entries(const Args &a, int row, int j0, int lane) {
+#pragma unroll
+        for (int c = 0; c < kAhead; c++) {
+            const int j = j0 + c * 32 + lane;
+            id[c] = j < a.k ? a.ids[(size_t)row * a.k + j] : -1;
+            t[c] = j < a.k ? a.teacher[(size_t)row * a.k + j] : 0.f;
+        }
+    }
+};
+
+// One warp: the record of a row.  `table`: slots that hold -1, and do so again afterwards.
+__device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, const Record &r, int *table, int *slot_of) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();                                // the record may be an earlier row's that a lane of this warp still reads
+    Ahead now = ahead;
+    ahead.ask(a, next_row);
+    const float weight = now.weight;
+    const float *x = a.x + (size_t)row * a.ld;
+    if (weight == 0.f) {
+        if (lane == 0) r.head->live = 0;
+        __syncwarp();
+        return;
+    }
+    const bool tail = a.teacher_lse != nullptr, soft = a.alpha != 1.f;
+    const int label = now.label < a.cols && now.label >= 0 ? now.label : -1;
+    const float x_label = label >= 0 ? x[label] : 0.f;
+    const double inv_t = 1.0 / (double)a.temperature, lse = now.lse;
+    float top = minus_inf(), anchor = minus_inf();
+    bool label_seen = false;
+    if (soft) {
+        // Of several entries with one id the first counts: the lowest lane of 32 at a time, and only if no earlier 32 had it.
+        for (int j0 = 0; j0 < a.k; j0 += 32 * kAhead) {
+            if (j0) now.entries(a, row, j0, lane);
+            float value[kAhead];
+#pragma unroll
+            for (int c = 0; c < kAhead; c++) {
+                if (now.id[c] >= a.cols || now.id[c] < 0) now.id[c] = -1;
+                value[c] = now.id[c] >= 0 ? x[now.id[c]] : 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < kAhead; c++) {
+                const int j = j0 + c * 32 + lane;
+                if (j - lane >= a.k) break;
+                int id = now.id[c], slot = -1;
+                const unsigned same = __match_any_sync(0xffffffffu, id);
+                if (id >= 0 && (int)__ffs(same) - 1 != lane) id = -1;
+                if (id >= 0 && a.k > 32) {
+                    unsigned h = ((unsigned)id * 2654435761u) >> 12 & (a.slots - 1);
+                    for (;;) {                   // the table is at most half full: an empty slot is met
+                        const int old = atomicCAS(table + h, -1, id);
+                        if (old == -1) { slot = (int)h; break; }
+                        if (old == id) { id = -1; break; }
+                        h = (h + 1) & (a.slots - 1);
+                    }
+                }
+                __syncwarp();
+                if (j < a.k) { r.id[j] = id; r.value[j] = value[c]; r.less[j] = now.t[c]; slot_of[j] = slot; }
+                if (id >= 0) { top = max_nan(top, now.t[c]); anchor = max_nan(anchor, value[c]); label_seen |= id == label; }
+            }
+        }
+        __syncwarp();
+        top = warp_max_nan(top); anchor = warp_max_nan(anchor);
+        if (!(fabsf(anchor) <= 3.4028235e38f)) anchor = 0.f;
+    }
+    const bool entries = soft && (tail || top != minus_inf());
+    const double ws = entries ? (double)weight * (1.0 - (double)a.alpha) * a.temperature : 0.0;
+    double sum = 0.0, terms = 0.0, per_sum = 1.0;
+    float z = 0.f, z1 = 0.f;
+    if (entries) {
+        for (int j = lane; j < a.k; j += 32) {
+            if (slot_of[j] >= 0) table[slot_of[j]] = -1;
+            if (r.id[j] < 0) continue;
+            double log_p;
+            float p;
+            if (tail) {                          // 1 - sum p may be small: in 64 bits up to the sum
+                log_p = (double)r.less[j] * inv_t - lse;
+                const double e = exp(log_p);
+                p = (float)e;
+                sum += e;
+                const float below = r.value[j] - anchor;
+                z += exp2_fast(below * (kLog2e / a.temperature)); z1 += exp2_fast(below * kLog2e);
+            } else {
+                const float d = (r.less[j] - top) * (float)inv_t;
+                log_p = d;
+                p = expf(d);
+                sum += p;
+            }
+            if (p != 0.f) terms += (double)p * (log_p - ((double)r.value[j] - (double)anchor) * inv_t);
+            r.less[j] = p;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, o); terms += __shfl_xor_sync(0xffffffffu, terms, o); }
+        if (tail) { z = warp_sum(z); z1 = warp_sum(z1); }
+        else per_sum = 1.0 / sum;
+        const float scale = (float)(ws * per_sum);
+        for (int j = lane; j < a.k; j += 32) r.less[j] *= scale;
+    } else if (soft) {
+        for (int j = lane; j < a.k; j += 32) { if (slot_of[j] >= 0) table[slot_of[j]] = -1; r.id[j] = -1; }
+    }
+    label_seen = __any_sync(0xffffffffu, entries && label_seen);
+    if (lane == 0) {
+        const double rest = tail && entries ? fmax(0.0, 1.0 - sum) : 0.0, wt = ws * a.temperature;
+        Head h;
+        h.hard = label >= 0 ? (double)weight * a.alpha : 0.0;
+        h.base = entries ? wt * (tail ? terms + (rest > 0.0 ? rest * logf((float)rest) : 0.0) : terms * per_sum - logf((float)sum)) : 0.0;
+        h.per_z = entries ? wt * (tail ? sum : 1.0) : 0.0;
+        h.per_rest = wt * rest;
+        h.inside = (float)(ws * (tail ? sum + rest : 1.0));
+        h.rest = (float)(ws * rest);
+        h.x_label = x_label; h.anchor = anchor; h.z = z; h.z1 = z1;
+        h.label = label; h.label_is_entry = label_seen; h.live = 1;
+        *r.head = h;
+    }
+    __syncwarp();
+}
+
+// Largest logit and sums of exponentials below it, of a thread, a warp, a row: z with the temperature (outside the entries where their cells are
+// -infinity), z1 without.
+struct Run {
+    float m, z, z1;
+    // relative to a common maximum; with nothing but -infinity so far the sums are zero and stay it
+    __device__ __forceinline__ void meet(float top, float c_t) {
+        const float d = m == top ? 0.f : m - top;
+        z *= exp2_fast(d * c_t); z1 *= exp2_fast(d * kLog2e);
+        m = top;
+    }
+};
+
+// TEAM threads share a row (or a piece of it): a warp of eight, or all warps of the block but the last.  CLUSTER: the pieces of a row are the blocks
+// of a cluster.  16-byte accesses whatever the row's alignment: the piece is laid out in shared memory with the alignment it has in
+// global memory, -infinity around it, so the sums need no bounds.  A thread copies (cp.async), sums and writes the same pieces of the row, so
+// between those steps nobody waits.  ex2 of one product: 2^-22 relative, the argument's roundings as in any fp32 softmax.
+constexpr int blocks_per_sm(int team) { return team == 32 ? 5 : team == 128 ? 8 : 3; }
+template <int TEAM, bool CLUSTER>
+__global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TEAM)) distill_kernel(const Args a) {
+    constexpr bool OWN = TEAM == 32;                       // every warp its own rows, entries and all
+    constexpr int TEAMS = OWN ? 8 : 1, W = TEAM / 32, RECORDS = OWN ? 1 : 3;
     extern __shared__ __align__(16) float smem[];
-    __shared__ double sums[TEAM == 32 ? 1 : 2 * kSums * W];
-    __shared__ double peers[CLUSTER ? 2 * kSums * kMaxCluster : 1];
-    const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM, lane = threadIdx.x & 31;
+    __shared__ Head heads[OWN ? 8 : 3];
+    __shared__ float4 runs[OWN ? 1 : 2][CLUSTER ? kMaxCluster : 1][W];
+    const int team = OWN ? threadIdx.x / 32 : 0, t = OWN ? threadIdx.x % 32 : threadIdx.x, lane = threadIdx.x & 31, warp = t >> 5;
     const int kk = (a.k + 3) & ~3;
-    float *x = smem + (size_t)team * (a.piece + 3 * kk);
-    float *value = x + a.piece, *prob = value + kk;        // of an entry in this piece: the student's logit, the teacher's weight
-    int *cell = reinterpret_cast<int *>(prob + kk);        // where in the piece it lies; -1: not an entry of this piece
+    float *x = smem + (size_t)team * (a.piece + 4 + (3 * RECORDS + 1) * kk + a.slots), *lists = x + a.piece + 4;
+    int *slot_of = reinterpret_cast<int *>(lists + 3 * RECORDS * kk), *table = slot_of + kk;
+    auto record = [&](int i) {
+        float *p = lists + 3 * kk * i;
+        return Record{heads + team + i, p, p + kk, reinterpret_cast<int *>(p + 2 * kk)};
+    };
     const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0, csize = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
     const int c0 = rank * a.piece, n = max(0, min(a.piece, a.cols - c0));
-    const float inv_t = 1.f / a.temperature;
-    const bool tail = a.teacher_lse != nullptr, soft = a.alpha != 1.f;
-    auto barrier = [&]() { if (TEAM == 32) __syncwarp(); else __syncthreads(); };
-    int flip = 0;
-    // v[0 .. COUNT) summed (or, LARGEST, the largest) over all threads that share the row, in a fixed order.  Two buffers take turns: one
-    // is written again only after the barrier of the exchange in between, which every reader has passed.
-    auto combine = [&](auto &v, auto largest) {
-        constexpr int COUNT = sizeof(v) / sizeof(double);
-        constexpr bool LARGEST = decltype(largest)::value;
-#pragma unroll
-        for (int i = 0; i < COUNT; i++)
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) { const double u = __shfl_xor_sync(0xffffffffu, v[i], o); v[i] = LARGEST ? max_nan(v[i], u) : v[i] + u; }
-        if (TEAM == 32) return;
-        double *b = sums + flip * (kSums * W);
-        if (lane == 0) {
-#pragma unroll
-            for (int i = 0; i < COUNT; i++) b[i * W + (threadIdx.x >> 5)] = v[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-            v[i] = b[i * W];
-            for (int w = 1; w < W; w++) v[i] = LARGEST ? max_nan(v[i], b[i * W + w]) : v[i] + b[i * W + w];
-        }
-        if (CLUSTER) {
-            cg::cluster_group cl = cg::this_cluster();
-            double *mine = peers + flip * (kSums * kMaxCluster);
-            if (threadIdx.x < (unsigned)csize) {
-                double *there = cl.map_shared_rank(mine, threadIdx.x);
-#pragma unroll
-                for (int i = 0; i < COUNT; i++) there[i * kMaxCluster + rank] = v[i];
-            }
-            cl.sync();
-#pragma unroll
-            for (int i = 0; i < COUNT; i++) {
-                v[i] = mine[i * kMaxCluster];
-                for (int c = 1; c < csize; c++) v[i] = LARGEST ? max_nan(v[i], mine[i * kMaxCluster + c]) : v[i] + mine[i * kMaxCluster + c];
-            }
-        }
-        flip ^= 1;
-    };
-    EB_GRID_WAIT();
+    const bool tail = a.teacher_lse != nullptr && a.alpha != 1.f, one_exp = a.temperature == 1.f, any_entries = a.alpha != 1.f;
+    const float c_t = kLog2e / a.temperature;
+    auto meeting = [&]() { if (CLUSTER) cg::this_cluster().sync(); else if (OWN) __syncwarp(); else __syncthreads(); };
+    auto team_barrier = [&]() { if (OWN) __syncwarp(); else asm volatile("bar.sync 1, %0;" ::"n"(TEAM) : "memory"); };
     const int first = (int)(blockIdx.x / csize) * TEAMS + team, step = (int)(gridDim.x / csize) * TEAMS;
-    for (int row = first; row < a.rows; row += step) {
-        const float weight = a.weights ? a.weights[row] : 1.f;
-        const float *src = a.x + (size_t)row * a.ld + c0;
-        float *dst = a.delta ? a.delta + (size_t)row * a.ld + c0 : nullptr;
-        // a row without weight, or without a single class that its mask leaves, adds nothing: its values are not looked at
-        bool empty = weight == 0.f;
-        double most[2] = {minus_inf(), minus_inf()};       // largest logit of the student, of the teacher's entries
-        int label = -1;
-        float x_label = 0.f;
-        if (!empty) {
-            float top = minus_inf(), t_top = minus_inf();
-            if (VEC) {
-#pragma unroll 4
-                for (int i = t * 4; i < n; i += TEAM * 4) {
-                    const float4 q = *reinterpret_cast<const float4 *>(src + i);
-                    *reinterpret_cast<float4 *>(x + i) = q;
-                    top = max_nan(max_nan(max_nan(q.x, q.y), max_nan(q.z, q.w)), top);
-                }
-            } else {
-#pragma unroll 4
-                for (int i = t; i < n; i += TEAM) { const float q = src[i]; x[i] = q; top = max_nan(top, q); }
-            }
-            if (a.alpha != 0.f) { label = a.labels[row]; if (label >= a.cols) label = -1; }
-            barrier();
-            if (t == 0 && label >= c0 && label < c0 + n) x_label = x[label - c0];
-            if (soft) {
-                // of several entries with the same id the first one counts: a cell holds the least number of an entry with its id
-                // until that one puts back what belongs there
-                for (int j = t; j < a.k; j += TEAM) {
-                    const int id = a.ids[(size_t)row * a.k + j], at = id >= c0 && id < c0 + n ? id - c0 : -1;
-                    cell[j] = at;
-                    if (at >= 0) value[j] = x[at];
-                }
-                barrier();
-                for (int j = t; j < a.k; j += TEAM) if (cell[j] >= 0) x[cell[j]] = __int_as_float(0x7fffffff);
-                barrier();
-                for (int j = t; j < a.k; j += TEAM) if (cell[j] >= 0) atomicMin(reinterpret_cast<int *>(x + cell[j]), j);
-                barrier();
-                for (int j = t; j < a.k; j += TEAM) {
-                    if (cell[j] < 0) continue;
-                    // only this thread changes cell[j]; the owner's number stays in the cell until the barrier below
-                    if (__float_as_int(x[cell[j]]) != j) { cell[j] = -1; continue; }
-                    prob[j] = a.teacher[(size_t)row * a.k + j];
-                    t_top = max_nan(t_top, prob[j]);
-                }
-                barrier();
-                for (int j = t; j < a.k; j += TEAM) if (cell[j] >= 0) x[cell[j]] = tail ? minus_inf() : value[j];
-            }
-            most[0] = top; most[1] = t_top;
-            combine(most, std::true_type());                          // its barrier lets every thread see the cells
-            if (TEAM == 32) __syncwarp();
-            empty = most[0] == (double)minus_inf();
+    if (OWN || warp == W) for (int i = lane; i < a.slots; i += 32) table[i] = -1;
+    __syncwarp();
+    EB_GRID_WAIT();
+
+    // the row's maximum and sums from its warps' lines; with the entries' cells closed the maximum is theirs too
+    auto combine = [&](int flip) {
+        Run run{minus_inf(), 0.f, 0.f};
+        for (int l = lane; l < csize * W; l += 32) {
+            const float4 q = runs[flip][l / W][l % W];
+            Run one{q.x, q.y, q.z};
+            const float top = max_nan(run.m, one.m);
+            run.meet(top, c_t); one.meet(top, c_t);
+            run.z += one.z; run.z1 += one.z1;
         }
-        if (empty) {
-            if (dst) for (int i = t; i < n; i += TEAM) dst[i] = 0.f;
-            if (rank == 0 && t == 0) a.loss[row] = 0.f;
-            barrier();
-            continue;
-        }
-        const float m = (float)most[0];
-        const bool ce = label >= 0, entries = soft && (tail || most[1] != (double)minus_inf());
-        // outside (all of the row unless `tail`), of the entries, with the temperature; the same without it; teacher's sum; KL terms; label
-        double v[6] = {0, 0, 0, 0, 0, x_label};
-        {
-            float zt = 0.f, z1 = 0.f;
-            for (int i = t; i < n; i += TEAM) {
-                const float d = x[i] - m;
-                if (entries) zt += expf(d * inv_t);
-                if (ce) z1 += expf(d);
+        run.meet(warp_max_nan(run.m), c_t);
+        run.z = warp_sum(run.z); run.z1 = warp_sum(run.z1);
+        return run;
+    };
+    auto add_entries = [&](Run &run, const Head &h) {
+        Run own{h.anchor, h.z, h.z1};
+        if (!tail || h.z == 0.f) own.m = minus_inf();
+        const float top = max_nan(run.m, own.m);
+        run.meet(top, c_t); own.meet(top, c_t);
+        return own;
+    };
+    auto loss_of = [&](const Head &h, const Run &run, const Run &own) {
+        const float z = run.z + own.z, z1 = one_exp && any_entries ? z : run.z1 + own.z1;
+        double l = h.base;
+        if (any_entries) l += h.per_z * (((double)run.m - (double)h.anchor) / (double)a.temperature + (double)logf(z));
+        if (h.per_rest > 0.0) l -= h.per_rest * ((double)logf(run.z) - (double)logf(z));
+        if (h.label >= 0) l += h.hard * ((double)run.m - (double)h.x_label + (double)logf(z1));
+        return (float)l;
+    };
+
+    if (!OWN && warp == W) {
+        // ============================ the entries, one row ahead; the loss ============================
+        Ahead ahead;
+        ahead.ask(a, first);
+        if (first < a.rows) look_up(a, first, first + step, ahead, record(0), table, slot_of);
+        meeting();
+        int i = 0, flip = 0;
+        for (int row = first; row < a.rows; row += step, flip ^= 1) {
+            const Head &h = *record(i).head;
+            // the record written here was last read two meetings ago
+            i = i == 2 ? 0 : i + 1;
+            if (row + step < a.rows) look_up(a, row + step, row + 2 * step, ahead, record(i), table, slot_of);
+            meeting();
+            if (rank) continue;
+            float loss = 0.f;
+            if (h.live) {
+                Run run = combine(flip);
+                const Run own = add_entries(run, h);
+                if (run.m != minus_inf()) loss = loss_of(h, run, own);
             }
-            v[0] = zt; v[2] = z1;
+            if (lane == 0) a.loss[row] = loss;
         }
-        if (entries) {
-            const double temperature = a.temperature, t_off = tail ? (double)a.teacher_lse[row] : most[1] / temperature;
-            for (int j = t; j < a.k; j += TEAM) {
-                if (cell[j] < 0) continue;
-                const double log_p = (double)prob[j] / temperature - t_off, log_q = ((double)value[j] - most[0]) / temperature, p = exp(log_p);
+    } else {
+        // piece v of the row, 16 bytes, on its way into its place; -infinity where there is no logit
+        auto fetch = [&](const float *src, int off, int end, int v) {
+            const int u = v * 4;
+            if (u >= off && u + 4 <= end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(x + u)), "l"(src - off + u) : "memory");
+            else {
+#pragma unroll
+                for (int q = 0; q < 4; q++) x[u + q] = u + q >= off && u + q < end ? src[u + q - off] : minus_inf();
+            }
+        };
+        auto source = [&](int row) { return a.x + (size_t)row * a.ld + c0; };
+        auto misfit = [&](const float *p) { return (int)((uintptr_t)p >> 2) & 3; };
+        auto fetch_row = [&](int row) {
+            if (row >= a.rows) return;
+            const float *src = source(row);
+            const int off = misfit(src), end = off + n;
+            for (int v = t; v * 4 < end; v += TEAM) fetch(src, off, end, v);
+        };
+        int i = 0, flip = 0;
+        Ahead ahead;
+        if (OWN) ahead.ask(a, first);
+        fetch_row(first);
+        if (!OWN) meeting();
+        for (int row = first; row < a.rows; row += step, flip ^= 1) {
+            const Record r = record(i);
+            if (OWN) look_up(a, row, row + step, ahead, r, table, slot_of);
+            else i = i == 2 ? 0 : i + 1;
+            float *dst = a.delta ? a.delta + (size_t)row * a.ld + c0 : nullptr;
+            const bool live = r.head->live != 0;
+            const int off = misfit(source(row)), end = off + n, nv = (end + 3) >> 2, label = live ? r.head->label : -1;
+            const bool ce = label >= 0;
+            Run run{minus_inf(), 0.f, 0.f};
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (live) {
                 if (tail) {
-                    v[1] += expf((value[j] - m) * inv_t);
-                    if (ce) v[2] += expf(value[j] - m);
+                    team_barrier();
+                    for (int j = t; j < a.k; j += TEAM) {
+                        const int at = r.id[j] - c0;
+                        if (r.id[j] >= 0 && at >= 0 && at < n) x[at + off] = minus_inf();
+                    }
+                    team_barrier();
                 }
-                v[3] += p;
-                if (p != 0.0) v[4] += p * (log_p - log_q);
-                prob[j] = (float)p;
+                auto add = [&](auto want_t, auto want_1) {
+#pragma unroll 2
+                    for (int v = t; v < nv; v += TEAM) {
+                        const float4 q = *reinterpret_cast<const float4 *>(x + v * 4);
+                        const float top = max_nan(max_nan(q.x, q.y), max_nan(q.z, q.w));
+                        if (!(top <= run.m)) run.meet(max_nan(top, run.m), c_t);
+                        const float m = run.m == minus_inf() ? 0.f : run.m;
+                        const float d0 = q.x - m, d1 = q.y - m, d2 = q.z - m, d3 = q.w - m;
+                        if (decltype(want_t)::value) run.z += (exp2_fast(d0 * c_t) + exp2_fast(d1 * c_t)) + (exp2_fast(d2 * c_t) + exp2_fast(d3 * c_t));
+                        if (decltype(want_1)::value) run.z1 += (exp2_fast(d0 * kLog2e) + exp2_fast(d1 * kLog2e)) + (exp2_fast(d2 * kLog2e) + exp2_fast(d3 * kLog2e));
+                    }
+                };
+                if (any_entries && ce && !one_exp) add(std::true_type(), std::true_type());
+                else if (any_entries) { add(std::true_type(), std::false_type()); run.z1 = run.z; }
+                else add(std::false_type(), std::true_type());
+                run.meet(warp_max_nan(run.m), c_t);
+                run.z = warp_sum(run.z); run.z1 = warp_sum(run.z1);
+                if (!OWN) {
+                    // a warp's line in every block of the cluster; the lines of two rows take turns
+                    float4 *mine = &runs[flip][rank][warp];
+                    if (CLUSTER) { if (lane < csize) *cg::this_cluster().map_shared_rank(mine, lane) = make_float4(run.m, run.z, run.z1, 0.f); }
+                    else if (lane == 0) *mine = make_float4(run.m, run.z, run.z1, 0.f);
+                }
             }
-        }
-        combine(v, std::false_type());
-        const double z = v[0] + v[1];
-        double kl = 0.0, inside = 0.0, outside = 0.0, p_scale = 0.0;      // factors of q_i at and outside the entries, of p_j
-        if (entries) {
-            if (tail) {
-                const double rest = fmax(0.0, 1.0 - v[3]), q_rest = v[0] / z;
-                kl = v[4] + v[3] * log(z) + (rest > 0.0 ? rest * log(rest / q_rest) : 0.0);
-                inside = v[3] + rest;
-                outside = q_rest > 0.0 ? inside - rest / q_rest : 0.0;
-                p_scale = 1.0;
-            } else {
-                kl = v[4] / v[3] - log(v[3]) + log(z);
-                inside = outside = 1.0;
-                p_scale = 1.0 / v[3];
+            if (!OWN) {
+                meeting();
+                if (live) run = combine(flip);
             }
-        }
-        const double ws = entries ? (double)weight * (1.0 - (double)a.alpha) * a.temperature : 0.0, wh = ce ? (double)weight * a.alpha : 0.0;
-        if (rank == 0 && t == 0) {
-            double l = 0.0;
-            if (entries) l += ws * a.temperature * kl;
-            if (ce) l += wh * (log(v[2]) - (v[5] - most[0]));
-            a.loss[row] = (float)l;
-        }
-        if (dst) {
-            const float f_in = entries ? (float)(ws * inside / z) : 0.f, f_out = entries ? (float)(ws * outside / z) : 0.f, f_p = (float)(ws * p_scale), f_1 = ce ? (float)(wh / v[2]) : 0.f;
-            for (int i = t; i < n; i += TEAM) {
-                const float d = x[i] - m;
-                float g = 0.f;
-                if (entries) g = f_out * expf(d * inv_t);
-                if (ce) g += f_1 * expf(d);
-                x[i] = g;
+            Run own{};
+            if (live) own = add_entries(run, *r.head);
+            if (!live || run.m == minus_inf()) {           // no weight, or a mask leaves nothing of the row
+                fetch_row(row + step);
+                if (dst) for (int q = t; q < n; q += TEAM) dst[q] = 0.f;
+                if (OWN && t == 0) a.loss[row] = 0.f;
+                continue;
             }
-            barrier();
-            if (entries)
+            if (OWN && t == 0) a.loss[row] = loss_of(*r.head, run, own);
+            if (!dst) { fetch_row(row + step); if (OWN) __syncwarp(); continue; }
+            const float m = run.m, z_out = run.z, z = z_out + own.z, z1 = one_exp && any_entries ? z : run.z1 + own.z1;
+            const float f_in = any_entries ? r.head->inside / z : 0.f, f_1 = ce ? (float)r.head->hard / z1 : 0.f;
+            const float f_out = tail ? (z_out > 0.f ? f_in - r.head->rest / z_out : 0.f) : f_in;
+            const bool straight = misfit(dst) == off;
+            // the next row's pieces follow this row's out of their places
+            const bool more = row + step < a.rows;
+            const float *next = source(more ? row + step : row);
+            const int next_off = misfit(next), next_end = more ? next_off + n : 0;
+            auto put = [&](auto want_t, auto want_1, float f) {
+#pragma unroll 2
+                for (int v = t; v < nv; v += TEAM) {
+                    const int u = v * 4;
+                    const float4 q = *reinterpret_cast<const float4 *>(x + u);
+                    const float d[4] = {q.x - m, q.y - m, q.z - m, q.w - m};
+                    float g[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        g[e] = f * exp2_fast(d[e] * (decltype(want_t)::value ? c_t : kLog2e));
+                        if (decltype(want_1)::value) g[e] = fmaf(f_1, exp2_fast(d[e] * kLog2e), g[e]);
+                    }
+                    if (straight && u >= off && u + 4 <= end) *reinterpret_cast<float4 *>(dst - off + u) = make_float4(g[0], g[1], g[2], g[3]);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) if (u + e >= off && u + e < end) dst[u + e - off] = g[e];
+                    }
+                    if (u < next_end) fetch(next, next_off, next_end, v);
+                }
+            };
+            if (any_entries && ce && !one_exp) put(std::true_type(), std::true_type(), f_out);
+            else if (any_entries) put(std::true_type(), std::false_type(), f_out + f_1);
+            else put(std::false_type(), std::false_type(), f_1);
+            if (nv * 4 < next_end && t == nv % TEAM) fetch(next, next_off, next_end, nv);      // a row that reaches one piece further
+            team_barrier();                                // the entries' and the label's places are written again, after the above
+            const float hard = (float)r.head->hard;
+            if (any_entries)
                 for (int j = t; j < a.k; j += TEAM) {
-                    if (cell[j] < 0) continue;
-                    const float d = value[j] - m;
-                    float g = f_in * expf(d * inv_t) - f_p * prob[j];
-                    if (ce) g += f_1 * expf(d);
-                    x[cell[j]] = g;
+                    const int at = r.id[j] - c0;
+                    if (r.id[j] < 0 || at < 0 || at >= n) continue;
+                    const float d = r.value[j] - m;
+                    float g = f_in * exp2_fast(d * c_t) - r.less[j];
+                    if (ce) g += f_1 * exp2_fast(d * kLog2e);
+                    if (r.id[j] == label) g -= hard;
+                    dst[at] = g;
                 }
-            barrier();
-            if (ce && t == 0 && label >= c0 && label < c0 + n) x[label - c0] -= (float)wh;
-            barrier();
-            if (VEC) for (int i = t * 4; i < n; i += TEAM * 4) *reinterpret_cast<float4 *>(dst + i) = *reinterpret_cast<const float4 *>(x + i);
-            else for (int i = t; i < n; i += TEAM) dst[i] = x[i];
+            if (ce && t == 0 && label >= c0 && label < c0 + n && !r.head->label_is_entry) {
+                const float d = r.head->x_label - m;
+                dst[label - c0] = f_1 * exp2_fast(d * kLog2e) + f_out * exp2_fast(d * c_t) - hard;
+            }
+            if (OWN) __syncwarp();
         }
-        barrier();
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    if (CLUSTER) cg::this_cluster().sync();                // a block's slots outlive the writes of the others
+    if (CLUSTER) cg::this_cluster().sync();                // a block's lines outlive the writes of the others
 }
 
 template <int TEAM, bool CLUSTER>
-int launch_distill(DevCtx *cx, int dev, cudaStream_t st, const Args &a, bool vec, unsigned csize, size_t smem) {
-    static bool configured[EDDLB200_MAX_DEVICES][2] = {};
-    auto kernel = vec ? distill_kernel<TEAM, true, CLUSTER> : distill_kernel<TEAM, false, CLUSTER>;
-    if (!configured[dev][vec]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+int launch_distill(DevCtx *cx, int dev, cudaStream_t st, const Args &a, unsigned csize, size_t smem) {
+    static bool configured[EDDLB200_MAX_DEVICES] = {};
+    auto kernel = distill_kernel<TEAM, CLUSTER>;
+    if (!configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
         if (e != cudaSuccess) return cuda_status(e, "distill(attributes)");
-        configured[dev][vec] = true;
+        configured[dev] = true;
     }
-    constexpr int block = TEAM == 32 ? 256 : TEAM, teams = TEAM == 32 ? 8 : 1;
-    size_t per_sm = (size_t)224 * 1024 / (smem + 5 * 1024);
-    if (per_sm > 2048 / block) per_sm = 2048 / block;
-    const size_t want = ceil_div(a.rows, teams), most = EDDLB200_NUM_SMS * per_sm / csize;
+    constexpr int block = TEAM == 32 ? 256 : TEAM + 32, teams = TEAM == 32 ? 8 : 1;
+    size_t per_sm = (size_t)227 * 1024 / (smem + 4 * 1024);
+    if (per_sm > (size_t)blocks_per_sm(TEAM)) per_sm = blocks_per_sm(TEAM);
+    if (per_sm < 1) per_sm = 1;
+    size_t most = EDDLB200_NUM_SMS * per_sm / csize;
+    if (CLUSTER) {
+        // The blocks of a cluster share a group of SMs, whose number need not divide by what they take: with more clusters than the GPU holds
+        // at once the rows of the last ones would wait for a whole round (1023 x 131071, 55 clusters of which 48 fit: 434 us, with 48 below).
+        static struct { size_t smem; int clusters; } held[EDDLB200_MAX_DEVICES][kMaxCluster + 1] = {};
+        auto &h = held[dev][csize];
+        if (h.smem != smem) {
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension; at[0].val.clusterDim.x = csize; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+            cudaLaunchConfig_t c = {};
+            c.gridDim = dim3((unsigned)(most * csize)); c.blockDim = dim3(block); c.dynamicSmemBytes = smem; c.attrs = at; c.numAttrs = 1;
+            int clusters = 0;
+            const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &c);
+            if (e != cudaSuccess) return cuda_status(e, "distill(clusters)");
+            h.smem = smem; h.clusters = clusters;
+        }
+        if ((size_t)h.clusters < most) most = h.clusters;
+        if (most < 1) return set_error(EDDLB200_ELIMIT, "distill: the device holds no cluster of %u blocks with %zu bytes each", csize, smem);
+    }
+    const size_t want = ceil_div(a.rows, teams);
     const unsigned clusters = (unsigned)(want < most ? want : most);
     if (CLUSTER) eb::launch_cluster(kernel, csize, clusters * csize, block, smem, st, a);
     else eb::launch(kernel, clusters, block, smem, st, a);
@@ -283,14 +488,14 @@ extern "C" int eddlb200_distill(int dev, const float *logits, const int *ids, co
     if (ld == (size_t)cols) EB_WRITES(delta, bytes); else EB_MODIFIES(delta, bytes);
     EB_WRITES(loss, each);
     ProfScope prof(cx, PROF_ELEMENTWISE, (delta ? 8.0 : 4.0) * rows * cols);
-    const bool vec = cols % 4 == 0 && ld % 4 == 0 && aligned16(logits) && aligned16(delta);
-    Args a{logits, teacher, teacher_lse, weights, ids, labels, loss, delta, rows, cols, k, 0, ld, temperature, alpha};
-    const size_t own = (size_t)3 * ((k + 3) & ~3);
-    auto pieces = [&](unsigned c) { a.piece = (int)((ceil_div(cols, c) + 3) & ~(size_t)3); return ((size_t)a.piece + own) * sizeof(float); };
-    if (cols <= 256) { const size_t smem = 8 * pieces(1); return launch_distill<32, false>(cx, dev, st, a, vec, 1, smem); }
-    if (cols <= 2048) { const size_t smem = pieces(1); return launch_distill<128, false>(cx, dev, st, a, vec, 1, smem); }
-    if (cols <= 16384) { const size_t smem = pieces(1); return launch_distill<512, false>(cx, dev, st, a, vec, 1, smem); }
+    Args a{logits, teacher, teacher_lse, weights, ids, labels, loss, delta, rows, cols, k, 0, 64, ld, temperature, alpha};
+    while (a.slots < 2 * k) a.slots *= 2;
+    const size_t kk = (k + 3) & ~3;
+    auto smem = [&](unsigned c, int records) { a.piece = (int)((ceil_div(cols, c) + 3) & ~(size_t)3); return ((size_t)a.piece + 4 + (3 * records + 1) * kk + a.slots) * sizeof(float); };
+    if (cols <= 256 || (cols <= 1024 && rows >= EDDLB200_NUM_SMS * 16)) { const size_t b = 8 * smem(1, 1); return launch_distill<32, false>(cx, dev, st, a, 1, b); }
+    if (cols <= 4096) { const size_t b = smem(1, 3); return launch_distill<128, false>(cx, dev, st, a, 1, b); }
+    if (cols <= 16384) { const size_t b = smem(1, 3); return launch_distill<256, false>(cx, dev, st, a, 1, b); }
     const unsigned csize = cols <= 32768 ? 2 : cols <= 65536 ? 4 : 8;
-    const size_t smem = pieces(csize);
-    return launch_distill<512, true>(cx, dev, st, a, vec, csize, smem);
+    const size_t b = smem(csize, 3);
+    return launch_distill<256, true>(cx, dev, st, a, csize, b);
 }

@@ -128,7 +128,7 @@ int eddlb200_cce_delta(int dev, const float *y_true, const float *y_pred, float 
 /* rows whose argmax(y_true) == argmax(y_pred), first maximum wins.  Blocking unless remembered (see above). */
 int eddlb200_accuracy(int dev, const float *y_true, const float *y_pred, int rows, int cols, int *host_out);
 
-/* Distillation (no counterpart in EDDL): loss of a student's logits [rows, cols] (rows `ld` floats apart, like delta's; at most 401408 columns)
+/* Distillation (no counterpart in EDDL): loss of a student's logits [rows, cols] (rows `ld` floats apart, like delta's; at most 344064 columns)
  * against the teacher's k <= 1024 best classes of each row -- ids [rows, k] and teacher [rows, k], the teacher's logits -- mixed with the
  * cross-entropy of hard labels [rows], and its gradient.  With x a row, q = softmax(x / T), T = temperature:
  *   loss[row] = w ((1 - alpha) T^2 KL + alpha (log sum exp x - x_label)),   delta = d loss[row] / d x
@@ -136,7 +136,7 @@ int eddlb200_accuracy(int dev, const float *y_true, const float *y_pred, int row
  *   else [rows], log sum exp(t / T) over ALL of the teacher's classes:  p_j = exp(teacher_j / T - teacher_lse), and p_r = max(0, 1 - sum p_j), the
  *          rest, is one class more: KL += p_r log(p_r / q_r), q_r the student's mass outside the entries
  * w = weights[row] (null: 1).  An id outside 0 .. cols - 1 is padding, of a repeated id the first entry counts; a label outside 0 .. cols - 1 has
- * no cross-entropy; a row of weight 0, or whose logits are all -infinity, has loss and delta 0 and nothing of a weightless row is read.  Logits of
+ * no cross-entropy; a row of weight 0, or whose logits are all -infinity, has loss and delta 0, whatever else it holds.  Logits of
  * -infinity are classes that are masked out.  labels may be null when alpha is 0; delta may be null, or logits itself.  delta's columns
  * from cols to ld keep what they hold. */
 int eddlb200_distill(int dev, const float *logits, const int *ids, const float *teacher, const float *teacher_lse, const int *labels,
