@@ -1,5 +1,6 @@
 // Dense algebra in 8-bit floating point with an fp32 scale for each block of 128 values along the reduction: quantisation of a
 // tensor in both of its directions, and the product of two quantised matrices on the tensor cores.
+#include <type_traits>
 #include <cuda_fp8.h>
 #include "tc_ptx.cuh"
 
@@ -339,6 +340,246 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, 1) fp8_product_kernel(
     if (warp == 1) tmem_dealloc(tmem, S::TMEM);
 }
 
+// ---- product of large matrices -------------------------------------------------------------------------------------------------
+// Pairs of CTAs (cta_group::2) that walk over tiles of 256 rows of P x 256 rows of Q: each CTA holds its own 128 rows of P and HALF of the rows of Q, so a
+// K-block moves 32 KB into each shared memory and is four instructions of 256 x 256 x 32 into one of two buffers of tensor memory.  Sixteen
+// epilogue warps, 32 lanes and 64 columns each, take a buffer out, scale it and add it to fp32 sums in registers while the next K-block
+// runs into the other one: four warps a scheduler hide the latencies between them (with eight warps of 128 columns the MMAs waited, 645 us).
+// What bounds it is power and operand traffic: 8192 x 8192 x 8192 takes 600 us, the GPU at its 1000 W and 1.5 GHz; the MMAs alone on operands that
+// are not copied 366 us at the same power, with the copies (64 KB a pair and K-block out of L2, 9 TB/s) 485.
+// Which operand is P is chosen so that scaling costs least: a matrix with a scale for 128 rows goes to the N side, where a warp's columns
+// share it, and an element takes one multiply-add; with a scale for every row on both sides the N side's are read from shared memory.
+// C's rows are P's rows here (ROWS) or Q's; in the first case a warp's values are turned through shared memory on their way out.
+// Registers: 640 threads are launched with 96 each; the copy and issue warps keep 56, the epilogue takes 104:
+// 128 x 56 + 512 x 104 = 60416 of 640 x 96 = 61440.
+constexpr int LG_STAGES = 5, LG_STAGE = 2 * 128 * kBlk, LG_THREADS = 640, LG_LINE = 32 * 17 * 4;
+constexpr int LG_SMEM = 1024 + LG_STAGES * LG_STAGE + 16 * LG_LINE;
+
+__device__ __forceinline__ void umma_fp8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 16 columns of the warp's lanes, not waited for
+__device__ __forceinline__ void tmem_ask16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+// the registers of the loads so far may be read: they pass through the wait, so that no use of them is moved ahead of it
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+}
+__device__ __forceinline__ void sts(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ float lds(uint32_t addr) { float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory"); return v; }
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+    float4 v; asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory"); return v;
+}
+
+template <bool VEC, bool ROWS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_product_large_kernel(const __grid_constant__ ProdParams P) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t lines = smem_u32(ring) + LG_STAGES * LG_STAGE;
+    __shared__ __align__(8) uint64_t bars[2 * LG_STAGES + 4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * LG_STAGES, bar_acc_full = bar_empty + 8 * LG_STAGES, bar_acc_empty = bar_acc_full + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1), kblocks = P.kblocks;
+    const int tiles_p = P.tiles_p, tiles = tiles_p * P.splits;         // splits: here the tiles along Q
+    // Tiles in bands of twelve along P, so that the pairs at work at a time share operands in L2 (8192 cubed: 600 us, in bands of eight 635).
+    auto place = [&](int tile, int &p0, int &q0) {
+        const int band = tile / (12 * P.splits), in = tile - band * 12 * P.splits, wide = min(12, tiles_p - band * 12);
+        p0 = (band * 12 + in % wide) * 256; q0 = in / wide * 256;
+    };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < LG_STAGES; s++) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
+        for (int s = 0; s < 2; s++) { mbar_init(bar_acc_full + 8 * s, 1); mbar_init(bar_acc_empty + 8 * s, 32); }
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_slot), 512);
+    EB_GRID_WAIT();
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive(); cluster_wait();                        // the other CTA's barriers are initialised before anything arrives on them
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    int fail = 0;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0 && elect_one()) {
+            // ============================ copies ============================
+            const uint32_t full_of_first = map_to_rank(bar_full, 0);
+            int s = 0, uses = 0; uint32_t phase = 1;
+            for (int tile = pair; tile < tiles && !fail; tile += pairs) {
+                int p0, q0;
+                place(tile, p0, q0);
+                for (int kb = 0; kb < kblocks; kb++) {
+                    if (!mbar_wait(bar_empty + 8 * s, phase, abort_flag)) { fail = 1; break; }
+                    if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * LG_STAGE);       // the bytes of both CTAs
+                    const uint32_t dst = smem_u32(ring) + s * LG_STAGE;
+                    tma_load_2d_pair(dst, &P.map_p, kb * kBlk, p0 + (int)rank * 128, full_of_first + 8 * s);
+                    tma_load_2d_pair(dst + 128 * kBlk, &P.map_q, kb * kBlk, q0 + (int)rank * 128, full_of_first + 8 * s);
+                    uses++;
+                    if (++s == LG_STAGES) { s = 0; phase ^= 1u; }
+                }
+            }
+            // the last arrivals on this CTA's barriers come from the other CTA: stay until they are in
+            for (int i = 0; i < LG_STAGES && i < uses && !fail; i++) {
+                if (--s < 0) { s = LG_STAGES - 1; phase ^= 1u; }
+                if (!mbar_wait(bar_empty + 8 * s, phase ^ 1u, abort_flag)) fail = 5;
+            }
+        } else if (warp == 1 && rank == 0 && elect_one()) {
+            // ============================ MMA issue ============================
+            int s = 0, buf = 0; uint32_t phase = 0, acc_phase = 1;
+            for (int tile = pair; tile < tiles && !fail; tile += pairs)
+                for (int kb = 0; kb < kblocks; kb++) {
+                    if (!mbar_wait(bar_full + 8 * s, phase, abort_flag)) { fail = 3; break; }
+                    if (!mbar_wait(bar_acc_empty + 8 * buf, acc_phase, abort_flag)) { fail = 2; break; }
+                    tc_fence_after();
+                    const uint64_t pd = make_desc(smem_u32(ring) + s * LG_STAGE), qd = make_desc(smem_u32(ring) + s * LG_STAGE + 128 * kBlk);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) umma_fp8_pair(tmem + buf * 256, pd + 2 * k, qd + 2 * k, P.idesc, k ? 1u : 0u);
+                    umma_commit_pair(bar_acc_full + 8 * buf);
+                    umma_commit_pair(bar_empty + 8 * s);
+                    if (++s == LG_STAGES) { s = 0; phase ^= 1u; }
+                    if (++buf == 2) { buf = 0; acc_phase ^= 1u; }
+                }
+        }
+        __syncwarp();
+    } else {
+        // ============================ epilogue ============================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int quarter = warp & 3, group = (warp - 4) >> 2;                 // 32 lanes, 64 columns
+        const uint32_t empty_of_first = map_to_rank(bar_acc_empty, 0);
+        const uint32_t line = lines + (warp - 4) * LG_LINE, from = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * 64);
+        uint32_t buf = 0, phase = 0;
+        for (int tile = pair; tile < tiles; tile += pairs) {
+            int p0, q0;
+            place(tile, p0, q0);
+            const int p = p0 + (int)rank * 128 + quarter * 32 + lane, q = q0 + group * 64;
+            const float *sp = P.scale_p + (min(p, P.p_rows - 1) >> P.p_shift), *sq = P.scale_q + (VEC ? min(q + lane, P.q_rows - 1) : min(q, P.q_rows - 1) >> 7);
+            const int second = VEC && q + 32 + lane < P.q_rows ? 32 : 0;                // a column past the last one takes another's scale: its products are zero
+            float acc[64];
+#pragma unroll
+            for (int i = 0; i < 64; i++) acc[i] = 0.f;
+            // scales of the next two K-blocks, on their way
+            float ahead_p[2], ahead_q[2][2];
+            int left = kblocks;                              // K-blocks whose scales have not been asked for
+            auto fetch = [&](int slot) {
+                if (--left < 0) return;
+                ahead_p[slot] = __ldg(sp);
+                ahead_q[slot][0] = __ldg(sq);
+                if (VEC) ahead_q[slot][1] = __ldg(sq + second);
+                sp += P.p_scales; sq += P.q_scales;
+            };
+            auto block = [&](int slot) {
+                const uint32_t scales = line + slot * 256;
+                const float s_p = VEC ? ahead_p[slot] : ahead_p[slot] * ahead_q[slot][0];
+                if (VEC) { sts(scales + lane * 4, ahead_q[slot][0]); sts(scales + 128 + lane * 4, ahead_q[slot][1]); }
+                fetch(slot);
+                if (!mbar_wait(bar_acc_full + 8 * buf, phase, abort_flag)) fail = 4;
+                if (__any_sync(0xffffffffu, fail)) { fail = 4; return; }
+                tc_fence_after();
+                const uint32_t base = from + buf * 256;
+                uint32_t r[2][16];
+                tmem_ask16(base, r[0]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    tmem_wait16(r[c & 1]);
+                    if (c < 3) tmem_ask16(base + 16 * (c + 1), r[(c + 1) & 1]);
+                    else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(empty_of_first + 8 * buf);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        float4 d = make_float4(__uint_as_float(r[c & 1][j]), __uint_as_float(r[c & 1][j + 1]), __uint_as_float(r[c & 1][j + 2]), __uint_as_float(r[c & 1][j + 3]));
+                        if (VEC) { const float4 s4 = lds4(scales + (c * 16 + j) * 4); d.x *= s4.x; d.y *= s4.y; d.z *= s4.z; d.w *= s4.w; }
+                        float *to = acc + c * 16 + j;
+                        to[0] = fmaf(d.x, s_p, to[0]); to[1] = fmaf(d.y, s_p, to[1]); to[2] = fmaf(d.z, s_p, to[2]); to[3] = fmaf(d.w, s_p, to[3]);
+                    }
+                }
+                buf ^= 1u;
+                if (!buf) phase ^= 1u;
+            };
+            fetch(0); fetch(1);
+#pragma unroll 1
+            for (int kb = kblocks; kb > 0 && !fail; kb -= 2) {
+                block(0);
+                if (kb > 1 && !fail) block(1);
+            }
+            if (fail) break;
+            if (ROWS) {
+                // C [p_rows][q_rows]: a lane holds a row's values, 32 rows x 16 columns at a time are turned
+                const int p_first = p0 + (int)rank * 128 + quarter * 32, rows = min(32, P.p_rows - p_first) - (lane >> 4);
+                auto out = [&](auto whole, auto inc) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) sts(line + (lane * 17 + j) * 4, acc[c * 16 + j]);
+                        __syncwarp();
+                        const int col = q + c * 16 + (lane & 15);
+                        float *dst = P.c + (size_t)(p_first + (lane >> 4)) * P.q_rows + col;
+                        if (col >= P.q_rows) continue;
+#pragma unroll 8
+                        for (int i = 0; i < 32; i += 2, dst += 2 * (size_t)P.q_rows) {
+                            if (!decltype(whole)::value && i >= rows) break;
+                            const float v = lds(line + ((i + (lane >> 4)) * 17 + (lane & 15)) * 4);
+                            *dst = decltype(inc)::value ? *dst + v : v;
+                        }
+                    }
+                };
+                if (P.inc) out(std::false_type(), std::true_type());
+                else if (p_first + 32 <= P.p_rows) out(std::true_type(), std::false_type());
+                else out(std::false_type(), std::false_type());
+                __syncwarp();
+            } else if (p < P.p_rows) {
+                // C [q_rows][p_rows]: the lanes are neighbours in memory
+                float *dst = P.c + (size_t)q * P.p_rows + p;
+                const int columns = P.q_rows - q;
+                if (!P.inc && columns >= 64) {
+#pragma unroll
+                    for (int i = 0; i < 64; i++, dst += P.p_rows) *dst = acc[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 64; i++, dst += P.p_rows) if (i < columns) *dst = P.inc ? *dst + acc[i] : acc[i];
+                }
+            }
+        }
+    }
+    if (fail) { *abort_flag = 1; atomicCAS(&g_fp8_status, 0, fail | warp << 8 | 7 << 16); }
+    tc_fence_before();
+    __syncthreads();
+    // both CTAs are done with each other's barriers, shared memory and accumulators
+    cluster_arrive(); cluster_wait();
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+template <bool VEC, bool ROWS>
+int launch_large(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P) {
+    static bool configured[EDDLB200_MAX_DEVICES] = {};
+    if (!configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(fp8_product_large_kernel<VEC, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SMEM);
+        if (e != cudaSuccess) return cuda_status(e, "fp8_mult2d(attributes)");
+        configured[dev] = true;
+    }
+    const int tiles = P.tiles_p * P.splits, pairs = tiles < EDDLB200_NUM_SMS / 2 ? tiles : EDDLB200_NUM_SMS / 2;
+    eb::launch(fp8_product_large_kernel<VEC, ROWS>, 2 * pairs, LG_THREADS, LG_SMEM, st, P);
+    EB_LAUNCH_CHECK("fp8_mult2d");
+    g_fp8_used[dev] = true;
+    return 0;
+}
+
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 // the driver entry point is looked up at run time: the library must load (and refuse work) on a machine without a driver
@@ -462,16 +703,32 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     }
     ProfScope prof(cx, PROF_GEMM, 2.0 * m * n * k);
     if (!k) return inc_c ? 0 : launch_zero_fill(cx, st, c, (size_t)m * n);
+    ProdParams P;
+    P.c = c; P.kblocks = (int)ceil_div(k, kBlk); P.inc = inc_c != 0;
+    struct Side { const void *q; size_t ld; const float *scale; int rows, block, format; };
+    const Side sa{qa, lda, scale_a, m, block_a, format_a}, sb{qb, ldb, scale_b, n, block_b, format_b};
+    auto sides = [&](const Side &p, const Side &q, int p_box, int q_box) {
+        P.scale_p = p.scale; P.scale_q = q.scale;
+        P.p_rows = p.rows; P.q_rows = q.rows;
+        P.p_shift = p.block == kBlk ? 7 : 0; P.q_shift = q.block == kBlk ? 7 : 0;
+        P.p_scales = (int)ceil_div(p.rows, p.block); P.q_scales = (int)ceil_div(q.rows, q.block);
+        return encode_bytes_map(&P.map_p, p.q, p.ld, p.rows, k, p_box) && encode_bytes_map(&P.map_q, q.q, q.ld, q.rows, k, q_box);
+    };
+    const char *const refused = "%s: the driver refuses a tensor map of the operands";
+    const size_t large = ceil_div(m, 256) * ceil_div(n, 256);
+    if (large >= EDDLB200_NUM_SMS / 4) {
+        const bool rows = block_b == kBlk, vec = !rows && block_a != kBlk;
+        if (large > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
+        if (!(rows ? sides(sa, sb, 128, 128) : sides(sb, sa, 128, 128))) return set_error(EDDLB200_EINVAL, refused, what);
+        P.tiles_p = (int)ceil_div(P.p_rows, 256); P.splits = (int)ceil_div(P.q_rows, 256);
+        P.idesc = rows ? fp8_idesc(format_a, format_b, 256, 256) : fp8_idesc(format_b, format_a, 256, 256);
+        return rows ? launch_large<false, true>(cx, dev, st, P) : vec ? launch_large<true, false>(cx, dev, st, P) : launch_large<false, false>(cx, dev, st, P);
+    }
     const int bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
     const size_t tiles_p = ceil_div(n, 128), tiles = tiles_p * ceil_div(m, bn);
     if (tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
-    ProdParams P;
-    if (!encode_bytes_map(&P.map_p, qb, ldb, n, k, 128) || !encode_bytes_map(&P.map_q, qa, lda, m, k, bn)) return set_error(EDDLB200_EINVAL, "%s: the driver refuses a tensor map of the operands", what);
-    P.scale_p = scale_b; P.scale_q = scale_a; P.c = c;
-    P.p_rows = n; P.q_rows = m; P.kblocks = (int)ceil_div(k, kBlk);
-    P.p_shift = block_b == kBlk ? 7 : 0; P.q_shift = block_a == kBlk ? 7 : 0;
-    P.p_scales = (int)ceil_div(n, block_b); P.q_scales = (int)ceil_div(m, block_a);
-    P.tiles_p = (int)tiles_p; P.inc = inc_c != 0;
+    if (!sides(sb, sa, 128, bn)) return set_error(EDDLB200_EINVAL, refused, what);
+    P.tiles_p = (int)tiles_p;
     size_t splits = EDDLB200_NUM_SMS / tiles;
     if (splits > 8) splits = 8;
     if (splits > (size_t)P.kblocks) splits = P.kblocks;

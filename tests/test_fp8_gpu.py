@@ -182,7 +182,15 @@ def test_product(lib, m, n, k, blocks, inc):
     check_product(lib, operand(lib, rng, m, k, E4M3, blocks[0]), operand(lib, rng, n, k, E4M3, blocks[1], up(k, 16) + 48), inc, rng)
 
 
-@pytest.mark.parametrize("m", [1, 24, 100, 300])
+# many tiles of 256 x 256: whole and ragged ones, one and several rounds of them, few and many K-blocks, an odd number of them
+@pytest.mark.parametrize("m,n,k", [(1537, 1601, 260), (300, 9601, 700), (9999, 130, 513), (2048, 1536, 128), (4096, 4352, 64), (1600, 1700, 2000)])
+@pytest.mark.parametrize("blocks", [(1, 128), (1, 1), (128, 128), (128, 1)])
+@pytest.mark.parametrize("inc", [0, 1])
+def test_large_product(lib, m, n, k, blocks, inc):
+    test_product(lib, m, n, k, blocks, inc)
+
+
+@pytest.mark.parametrize("m", [1, 24, 100, 300, 9000])
 @pytest.mark.parametrize("formats", [(E4M3, E5M2), (E5M2, E4M3), (E5M2, E5M2)])
 def test_product_formats(lib, m, formats):
     rng = np.random.default_rng(m)
