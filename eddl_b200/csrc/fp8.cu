@@ -12,9 +12,10 @@ constexpr int kBlk = 128;
 
 // ---- quantisation ------------------------------------------------------------------------------------------------------------
 // One block per 128 x 128 tile, one read of it for both directions; bound by memory (4 bytes read, 1 or 2 written a value).  A warp
-// takes 16 rows, a lane four columns of each, so a row's 128 values are one 512-byte access and their largest magnitude one warp
-// reduction; the columns' come from the warps' through shared memory.  The transpose goes through a 16 KB byte tile (16-byte pieces,
-// swizzled so that neither side has bank conflicts) and leaves in 128-byte lines.
+// takes eight rows, a lane four columns of each, so a row's 128 values are one 512-byte access and their largest magnitude one warp
+// reduction; the columns' come from the warps' through shared memory.  A scale is worked out by one lane (of a row) or thread (of a
+// column) and handed to the others: a division a value would cost more than the copy.  The transpose goes through a 16 KB byte tile (8-byte
+// pieces, swizzled so that neither side has bank conflicts to speak of) and leaves in 128-byte lines.
 struct QuantArgs {
     const float *a;
     uint8_t *q, *qt;
@@ -44,20 +45,18 @@ __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
     const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, kind), hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, kind);
     return lo | hi << 16;
 }
-// magnitude as bits, in which larger numbers are larger; a NaN counts as nothing
-__device__ __forceinline__ unsigned magnitude(float v) { const unsigned b = __float_as_uint(v) & 0x7fffffffu; return b > 0x7f800000u ? 0u : b; }
-
 template <int FORMAT, bool TILE, bool VEC>
-__global__ void __launch_bounds__(256, 2) fp8_quantize_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(512, 2) fp8_quantize_kernel(const QuantArgs a) {
     EB_GRID_WAIT();
-    __shared__ unsigned col_peak[8][kBlk];
+    constexpr int WARPS = 16, ROWS = kBlk / WARPS;
+    __shared__ float col_peak[WARPS][kBlk], col_factor[kBlk];
     __shared__ __align__(16) uint8_t turned[kBlk * kBlk];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tx = blockIdx.x % a.tiles_x, ty = blockIdx.x / a.tiles_x;
-    const int r0 = ty * kBlk + warp * 16, c0 = tx * kBlk + lane * 4;
-    float v[16][4];
+    const int r0 = ty * kBlk + warp * ROWS, c0 = tx * kBlk + lane * 4;
+    float v[ROWS][4];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int i = 0; i < ROWS; i++) {
         const float *src = a.a + (size_t)(r0 + i) * a.cols + c0;
         const bool row = r0 + i < a.rows;
         if (VEC) {
@@ -68,66 +67,83 @@ __global__ void __launch_bounds__(256, 2) fp8_quantize_kernel(const QuantArgs a)
             for (int j = 0; j < 4; j++) v[i][j] = row && c0 + j < a.cols ? src[j] : 0.f;
         }
     }
-    unsigned mine[4] = {0, 0, 0, 0};                                   // of the lane's columns over the warp's rows
+    // largest magnitudes; fmaxf leaves a NaN out
     if (TILE || a.qt) {
+        float mine[4] = {0.f, 0.f, 0.f, 0.f};                          // of the lane's columns over the warp's rows
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) mine[j] = max(mine[j], magnitude(v[i][j]));
-        *reinterpret_cast<uint4 *>(&col_peak[warp][lane * 4]) = make_uint4(mine[0], mine[1], mine[2], mine[3]);
+            for (int j = 0; j < 4; j++) mine[j] = fmaxf(mine[j], fabsf(v[i][j]));
+        *reinterpret_cast<float4 *>(&col_peak[warp][lane * 4]) = make_float4(mine[0], mine[1], mine[2], mine[3]);
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 8; w++) {
-            const uint4 p = *reinterpret_cast<const uint4 *>(&col_peak[w][lane * 4]);
-            mine[0] = max(mine[0], p.x); mine[1] = max(mine[1], p.y); mine[2] = max(mine[2], p.z); mine[3] = max(mine[3], p.w);
-        }
     }
     Scale tile{0.f, 0.f};
     if (TILE) {
-        tile = scale_of<FORMAT>(__reduce_max_sync(0xffffffffu, max(max(mine[0], mine[1]), max(mine[2], mine[3]))), a.pow2);
+        // every warp looks through the columns of all
+        float peak = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float4 p = *reinterpret_cast<const float4 *>(&col_peak[w][lane * 4]);
+            peak = fmaxf(peak, fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w)));
+        }
+        tile = scale_of<FORMAT>(__reduce_max_sync(0xffffffffu, __float_as_uint(peak)), a.pow2);
         if (threadIdx.x == 0) {
             const int row_blocks = (a.rows + kBlk - 1) / kBlk;
             if (a.q) a.scale[(size_t)tx * row_blocks + ty] = tile.scale;
             if (a.qt) a.scale_t[(size_t)ty * a.tiles_x + tx] = tile.scale;
         }
+    } else if (a.qt && threadIdx.x < kBlk) {
+        float peak = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) peak = fmaxf(peak, col_peak[w][threadIdx.x]);
+        const Scale s = scale_of<FORMAT>(__float_as_uint(peak), a.pow2);
+        col_factor[threadIdx.x] = s.factor;
+        if (tx * kBlk + (int)threadIdx.x < a.cols) a.scale_t[(size_t)ty * a.cols + tx * kBlk + threadIdx.x] = s.scale;
     }
     if (a.q) {
-        float own_scale = 0.f;
+        Scale own = tile;                                              // of row `lane`
+        if (!TILE) {
+            unsigned peak = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            Scale s = tile;
-            if (!TILE) {
-                s = scale_of<FORMAT>(__reduce_max_sync(0xffffffffu, max(max(magnitude(v[i][0]), magnitude(v[i][1])), max(magnitude(v[i][2]), magnitude(v[i][3])))), a.pow2);
-                if (lane == i) own_scale = s.scale;
+            for (int i = 0; i < ROWS; i++) {
+                const unsigned of_row = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fmaxf(0.f, fabsf(v[i][0])), fabsf(v[i][1])), fmaxf(fabsf(v[i][2]), fabsf(v[i][3])))));
+                if (lane == i) peak = of_row;
             }
+            own = scale_of<FORMAT>(peak, a.pow2);
+            if (lane < ROWS && r0 + lane < a.rows) a.scale[(size_t)tx * a.rows + r0 + lane] = own.scale;
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            const float f = TILE ? tile.factor : __shfl_sync(0xffffffffu, own.factor, i);
             if (r0 + i >= a.rows || c0 >= a.cols) continue;
-            const unsigned bytes = pack4<FORMAT>(__fmul_rn(v[i][0], s.factor), __fmul_rn(v[i][1], s.factor), __fmul_rn(v[i][2], s.factor), __fmul_rn(v[i][3], s.factor));
+            const unsigned bytes = pack4<FORMAT>(__fmul_rn(v[i][0], f), __fmul_rn(v[i][1], f), __fmul_rn(v[i][2], f), __fmul_rn(v[i][3], f));
             uint8_t *dst = a.q + (size_t)(r0 + i) * a.ldq + c0;
             if (VEC || c0 + 4 <= a.cols) *reinterpret_cast<unsigned *>(dst) = bytes;
             else for (int j = 0; c0 + j < a.cols; j++) dst[j] = (uint8_t)(bytes >> 8 * j);
         }
-        if (!TILE && lane < 16 && r0 + lane < a.rows) a.scale[(size_t)tx * a.rows + r0 + lane] = own_scale;
     }
     if (!a.qt) return;
+    float4 factor = make_float4(tile.factor, tile.factor, tile.factor, tile.factor);
+    if (!TILE) {
+        __syncthreads();
+        factor = *reinterpret_cast<const float4 *>(&col_factor[lane * 4]);
+    }
+    const float each[4] = {factor.x, factor.y, factor.z, factor.w};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        Scale s = tile;
-        if (!TILE) {
-            s = scale_of<FORMAT>(mine[j], a.pow2);
-            if (warp == 0 && c0 + j < a.cols) a.scale_t[(size_t)ty * a.cols + c0 + j] = s.scale;
-        }
-        unsigned b[4];
+        unsigned b[2];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            b[i] = pack4<FORMAT>(__fmul_rn(v[4 * i][j], s.factor), __fmul_rn(v[4 * i + 1][j], s.factor), __fmul_rn(v[4 * i + 2][j], s.factor), __fmul_rn(v[4 * i + 3][j], s.factor));
-        *reinterpret_cast<uint4 *>(turned + (lane * 4 + j) * kBlk + ((warp ^ lane) & 7) * 16) = make_uint4(b[0], b[1], b[2], b[3]);
+        for (int i = 0; i < 2; i++)
+            b[i] = pack4<FORMAT>(__fmul_rn(v[4 * i][j], each[j]), __fmul_rn(v[4 * i + 1][j], each[j]), __fmul_rn(v[4 * i + 2][j], each[j]), __fmul_rn(v[4 * i + 3][j], each[j]));
+        // row lane * 4 + j of the turned tile, bytes warp * 8 ..: 16-byte piece warp / 2 lies at piece (warp / 2) ^ (lane & 7)
+        *reinterpret_cast<uint2 *>(turned + (lane * 4 + j) * kBlk + (((warp >> 1) ^ lane) & 7) * 16 + (warp & 1) * 8) = make_uint2(b[0], b[1]);
     }
     __syncthreads();
     const int at = (threadIdx.x & 7) * 16, left = a.rows - ty * kBlk - at;            // bytes of this piece that are there
     if (left <= 0) return;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int col = (int)(threadIdx.x >> 3) + 32 * i, gc = tx * kBlk + col;
+    for (int i = 0; i < 2; i++) {
+        const int col = (int)(threadIdx.x >> 3) + 64 * i, gc = tx * kBlk + col;
         if (gc >= a.cols) break;
         const uint8_t *src = turned + col * kBlk + (((threadIdx.x & 7) ^ (col >> 2)) & 7) * 16;
         uint8_t *dst = a.qt + (size_t)gc * a.ldqt + (size_t)ty * kBlk + at;
@@ -163,15 +179,18 @@ struct ProdParams {
 __device__ int g_fp8_status;
 bool g_fp8_used[EDDLB200_MAX_DEVICES] = {};
 
+// Up to 64 rows of Q two blocks share an SM: the chain copy -> MMA -> epilogue of one K-block is long and its work short, so what counts is how many
+// K-blocks are on their way (tensor memory holds BUFS of them a block).
 template <int BN>
 struct ProdShape {
-    static constexpr int EPI = BN >= 64 ? 8 : 4, THREADS = 64 + EPI * 32, COLS = BN / (EPI / 4);
-    static constexpr int STAGE = 128 * kBlk + BN * kBlk, STAGES = 196608 / STAGE < 8 ? 196608 / STAGE : 8;
-    static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int EPI = BN >= 64 ? 8 : 4, THREADS = 64 + EPI * 32, COLS = BN / (EPI / 4), PER_SM = BN <= 64 ? 2 : 1;
+    static constexpr int STAGE = 128 * kBlk + BN * kBlk, STAGES = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : BN == 128 ? 6 : 4;
+    static constexpr int BUFS = BN <= 32 ? 8 : BN == 256 ? 2 : 4, TMEM = BUFS * BN;
     static constexpr int PER_LANE = (COLS + 31) / 32;
     static constexpr int SCALES = EPI * 2 * PER_LANE * 32 * 4;
     static constexpr int SMEM = 1024 + STAGES * STAGE + SCALES;
     static_assert(STAGES * STAGE >= BN * 512, "the partial tile of a split takes the place of the operands");
+    static_assert(PER_SM * TMEM <= 512 && PER_SM * (SMEM + 2048) <= 228 * 1024, "blocks of one SM");
 };
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const CUtensorMap *map, int x, int y, uint32_t bar) {
@@ -182,29 +201,35 @@ __device__ __forceinline__ void umma_fp8(uint32_t d_tmem, uint64_t adesc, uint64
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
+// four values at this address in the shared memory of the cluster's block `rank`
+__device__ __forceinline__ float4 lds4_of(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_to_rank(addr, rank)) : "memory");
+    return v;
+}
 // fp32 sums, both operands K-major; formats: 0 = e4m3, 1 = e5m2
 constexpr unsigned fp8_idesc(int format_a, int format_b, int m, int n) {
     return (1u << 4) | (unsigned)format_a << 7 | (unsigned)format_b << 10 | (unsigned)(n >> 3) << 17 | (unsigned)(m >> 4) << 24;
 }
 
 template <int BN>
-__global__ void __launch_bounds__(ProdShape<BN>::THREADS, 1) fp8_product_kernel(const __grid_constant__ ProdParams P) {
+__global__ void __launch_bounds__(ProdShape<BN>::THREADS, ProdShape<BN>::PER_SM) fp8_product_kernel(const __grid_constant__ ProdParams P) {
     using S = ProdShape<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float *scales = (float *)(ring + S::STAGES * S::STAGE);
-    __shared__ __align__(8) uint64_t bars[2 * S::STAGES + 4];
+    __shared__ __align__(8) uint64_t bars[2 * S::STAGES + 2 * S::BUFS];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
-    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES, bar_acc_full = bar_empty + 8 * S::STAGES, bar_acc_empty = bar_acc_full + 16;
+    const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::STAGES, bar_acc_full = bar_empty + 8 * S::STAGES, bar_acc_empty = bar_acc_full + 8 * S::BUFS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = (int)(blockIdx.x % P.splits), tile = (int)(blockIdx.x / P.splits);
     const int p0 = (tile % P.tiles_p) * 128, q0 = (tile / P.tiles_p) * BN;
     const int kb0 = (int)((long long)P.kblocks * split / P.splits), kb1 = (int)((long long)P.kblocks * (split + 1) / P.splits);
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
-        for (int s = 0; s < 2; s++) { mbar_init(bar_acc_full + 8 * s, 1); mbar_init(bar_acc_empty + 8 * s, S::EPI); }
+        for (int s = 0; s < S::BUFS; s++) { mbar_init(bar_acc_full + 8 * s, 1); mbar_init(bar_acc_empty + 8 * s, S::EPI); }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -248,7 +273,7 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, 1) fp8_product_kernel(
                 umma_commit(bar_empty + 8 * s);
                 umma_commit(bar_acc_full + 8 * buf);
                 if (++s == S::STAGES) { s = 0; phase ^= 1u; }
-                if (++buf == 2) { buf = 0; acc_phase ^= 1u; }
+                if (++buf == S::BUFS) { buf = 0; acc_phase ^= 1u; }
             }
         }
         __syncwarp();
@@ -270,7 +295,7 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, 1) fp8_product_kernel(
         fetch(kb0);
         int buf = 0; uint32_t phase = 0;
         for (int kb = kb0; kb < kb1; kb++) {
-            float *line = mine + (buf * S::PER_LANE) * 32;
+            float *line = mine + ((buf & 1) * S::PER_LANE) * 32;
 #pragma unroll
             for (int i = 0; i < S::PER_LANE; i++) line[i * 32 + lane] = next_q[i];
             const float s_p = next_p;
@@ -295,7 +320,7 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, 1) fp8_product_kernel(
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_acc_empty + 8 * buf);
-            if (++buf == 2) { buf = 0; phase ^= 1u; }
+            if (++buf == S::BUFS) { buf = 0; phase ^= 1u; }
         }
         if (P.splits == 1) {
             float *dst = P.c + (size_t)q * P.p_rows + p;
@@ -319,17 +344,25 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, 1) fp8_product_kernel(
         __syncwarp();
         cluster_arrive(); cluster_wait();
         if (warp >= 2) {
-            const int column = (threadIdx.x - 64) & 127, p = p0 + column;
-            for (int i = split + P.splits * ((threadIdx.x - 64) >> 7); i < BN && q0 + i < P.q_rows; i += P.splits * (S::EPI / 4)) {
-                float sum = 0.f;
-                for (int r = 0; r < P.splits; r++) {
-                    float v;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(ring) + (i * 128 + column) * 4, r)));
-                    sum += v;
-                }
-                if (p < P.p_rows) {
-                    float *at = P.c + (size_t)(q0 + i) * P.p_rows + p;
-                    *at = P.inc ? *at + sum : sum;
+            // a warp a row of C at a time, a lane four neighbouring values: its loads from all blocks are on their way together
+            const int p = p0 + lane * 4;
+            const bool straight = P.p_rows % 4 == 0 && aligned16(P.c);
+#pragma unroll 2
+            for (int i = split + P.splits * (warp - 2); i < BN && q0 + i < P.q_rows; i += P.splits * S::EPI) {
+                float4 v[8];
+#pragma unroll
+                for (int r = 0; r < 8; r++) if (r < P.splits) v[r] = lds4_of(smem_u32(ring) + (i * 128 + lane * 4) * 4, r);
+                float4 sum = v[0];
+#pragma unroll
+                for (int r = 1; r < 8; r++) if (r < P.splits) { sum.x += v[r].x; sum.y += v[r].y; sum.z += v[r].z; sum.w += v[r].w; }
+                float *at = P.c + (size_t)(q0 + i) * P.p_rows + p;
+                if (straight && p < P.p_rows) {
+                    if (P.inc) { const float4 o = *reinterpret_cast<const float4 *>(at); sum.x += o.x; sum.y += o.y; sum.z += o.z; sum.w += o.w; }
+                    *reinterpret_cast<float4 *>(at) = sum;
+                } else {
+                    const float each[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) if (p + k < P.p_rows) at[k] = P.inc ? at[k] + each[k] : each[k];
                 }
             }
         }
@@ -618,6 +651,31 @@ int launch_product(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P, un
     return 0;
 }
 
+// Which kernel, tile and split: the least estimated time, in cycles of an SM.  The figures are fitted to a sweep of 19 shapes from 1 x 1024 x 1024 to
+// 1024 x 4096 x 4096 over all tiles and splits; the estimates are within 20 % of it.  A K-block costs an SM its operands' way through L2 or, in the
+// wide tiles, the epilogue's; alone on its SM a block waits at least for its own chain.  A tile costs its start and its stores and, when split,
+// the exchange between the blocks of a cluster.  256 x 4096 x 4096: 128 rows in two splits 15.8 us, pairs 22.0; 2048 cubed: pairs 16.0, 256 rows 24.8.
+struct Plan { int bn = 0, splits = 1; size_t tiles = 0; };           // bn 0: the kernel on pairs of CTAs
+Plan pick_plan(int m, int n, int kblocks) {
+    Plan best;
+    best.tiles = ceil_div(m, 256) * ceil_div(n, 256);
+    double least = (double)ceil_div(best.tiles, (size_t)EDDLB200_NUM_SMS / 2) * (1050.0 * kblocks + 8000.0);
+    for (int bn = 16; bn <= 256; bn *= 2) {
+        if (bn > 16 && bn / 2 >= m) break;                           // half of the tile would be empty
+        const size_t tiles = ceil_div(n, 128) * ceil_div(m, bn), slots = (size_t)EDDLB200_NUM_SMS * (bn <= 64 ? 2 : 1);
+        const double block = bn == 16 ? 410.0 : bn == 32 ? 450.0 : bn == 64 ? 580.0 : bn == 128 ? 950.0 : 1800.0;
+        const double alone = bn == 16 ? 600.0 : bn == 32 ? 720.0 : bn == 64 ? 950.0 : block;
+        for (int splits = 1; splits <= 8 && splits <= kblocks; splits++) {
+            const size_t jobs = tiles * splits, rounds = ceil_div(jobs, slots), on_one = ceil_div(jobs, (size_t)EDDLB200_NUM_SMS);
+            const double each = (double)ceil_div(kblocks, splits);
+            const double work = on_one > 1 ? on_one * each * block : each * alone;
+            const double t = work + rounds * (4000.0 + 25.0 * bn + (splits > 1 ? 700.0 * splits + 8.0 * bn : 0.0));
+            if (t < least) { least = t; best.bn = bn; best.splits = splits; best.tiles = tiles; }
+        }
+    }
+    return best;
+}
+
 size_t matrix_bytes(int rows, int cols, size_t ld) { return rows && cols ? (size_t)(rows - 1) * ld + cols : 0; }
 size_t scale_bytes(int rows, int cols, int block_rows) { return ceil_div(cols, kBlk) * ceil_div(rows, block_rows) * sizeof(float); }
 
@@ -671,7 +729,7 @@ int eddlb200_fp8_quantize(int dev, const float *a, int rows, int cols, int forma
     const QuantArgs args{a, (uint8_t *)q, (uint8_t *)qt, scale, scale_t, ldq, ldqt, rows, cols, (int)ceil_div(cols, kBlk), pow2};
     const bool vec = cols % 4 == 0 && aligned16(a);
     auto kernel = format == EDDLB200_E4M3 ? quantize_kernel<EDDLB200_E4M3>(block_rows == kBlk, vec) : quantize_kernel<EDDLB200_E5M2>(block_rows == kBlk, vec);
-    eb::launch(kernel, (unsigned)tiles, 256, 0, st, args);
+    eb::launch(kernel, (unsigned)tiles, 512, 0, st, args);
     EB_LAUNCH_CHECK(what);
     return 0;
 }
@@ -715,31 +773,25 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
         return encode_bytes_map(&P.map_p, p.q, p.ld, p.rows, k, p_box) && encode_bytes_map(&P.map_q, q.q, q.ld, q.rows, k, q_box);
     };
     const char *const refused = "%s: the driver refuses a tensor map of the operands";
-    const size_t large = ceil_div(m, 256) * ceil_div(n, 256);
-    if (large >= EDDLB200_NUM_SMS / 4) {
+    const Plan plan = pick_plan(m, n, P.kblocks);
+    if (plan.tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
+    if (!plan.bn) {
         const bool rows = block_b == kBlk, vec = !rows && block_a != kBlk;
-        if (large > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
         if (!(rows ? sides(sa, sb, 128, 128) : sides(sb, sa, 128, 128))) return set_error(EDDLB200_EINVAL, refused, what);
         P.tiles_p = (int)ceil_div(P.p_rows, 256); P.splits = (int)ceil_div(P.q_rows, 256);
         P.idesc = rows ? fp8_idesc(format_a, format_b, 256, 256) : fp8_idesc(format_b, format_a, 256, 256);
         return rows ? launch_large<false, true>(cx, dev, st, P) : vec ? launch_large<true, false>(cx, dev, st, P) : launch_large<false, false>(cx, dev, st, P);
     }
-    const int bn = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256;
-    const size_t tiles_p = ceil_div(n, 128), tiles = tiles_p * ceil_div(m, bn);
-    if (tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
+    const int bn = plan.bn;
     if (!sides(sb, sa, 128, bn)) return set_error(EDDLB200_EINVAL, refused, what);
-    P.tiles_p = (int)tiles_p;
-    size_t splits = EDDLB200_NUM_SMS / tiles;
-    if (splits > 8) splits = 8;
-    if (splits > (size_t)P.kblocks) splits = P.kblocks;
-    P.splits = (int)(splits < 1 ? 1 : splits);
+    P.tiles_p = (int)ceil_div(n, 128); P.splits = plan.splits;
     P.idesc = fp8_idesc(format_b, format_a, 128, bn);
     switch (bn) {
-        case 16: return launch_product<16>(cx, dev, st, P, (unsigned)tiles);
-        case 32: return launch_product<32>(cx, dev, st, P, (unsigned)tiles);
-        case 64: return launch_product<64>(cx, dev, st, P, (unsigned)tiles);
-        case 128: return launch_product<128>(cx, dev, st, P, (unsigned)tiles);
-        default: return launch_product<256>(cx, dev, st, P, (unsigned)tiles);
+        case 16: return launch_product<16>(cx, dev, st, P, (unsigned)plan.tiles);
+        case 32: return launch_product<32>(cx, dev, st, P, (unsigned)plan.tiles);
+        case 64: return launch_product<64>(cx, dev, st, P, (unsigned)plan.tiles);
+        case 128: return launch_product<128>(cx, dev, st, P, (unsigned)plan.tiles);
+        default: return launch_product<256>(cx, dev, st, P, (unsigned)plan.tiles);
     }
 }
 
