@@ -16,28 +16,46 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxCols = 16384;            // 1024 threads with four 16-byte pieces each; four blocks of 512 with two each
 
-// Sums of K values over a team of TPR threads (a warp, or the whole block); every thread gets them.  Two buffers take turns, so one
-// barrier is enough: a buffer is written again only after the barrier of the sums in between, which every reader has passed.
+// Sums of K values over a team of TPR threads (a warp, or the whole block); every thread gets them, added in a fixed order.  K is a power of two:
+// the lanes halve the number of values they carry with each of the first exchanges, so K sums of a warp cost K + 1 shuffles or so, not 5 K.
+// Two buffers take turns, so one barrier is enough: a buffer is written again only after the barrier of the sums in between,
+// which every reader has passed.
 template <int TPR, int K>
 struct TeamSum {
-    static constexpr int W = TPR / 32;
+    static constexpr int W = TPR / 32, LANES = 32 / K;                  // LANES: neighbours that end up with the same sum
+    static_assert((K & (K - 1)) == 0 && K <= 8 && W <= 32, "");
     float *buf;
     int flip = 0;
     __device__ __forceinline__ TeamSum(float *b) : buf(b) {}
     __device__ __forceinline__ void operator()(float (&v)[K]) {
-#pragma unroll
-        for (int k = 0; k < K; k++) v[k] = warp_sum(v[k]);
-        if (TPR == 32) return;
-        float *b = buf + flip * (K * W);
-        flip ^= 1;
         const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-        if (lane == 0) {
+        // after the exchange over `o` lanes a lane holds the values whose number has, in that place, the lane's bit
 #pragma unroll
-            for (int k = 0; k < K; k++) b[k * W + w] = v[k];
+        for (int half = K / 2, o = 16; half > 0; half /= 2, o /= 2) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int k = 0; k < half; k++) {
+                const float give = up ? v[k] : v[k + half], keep = up ? v[k + half] : v[k];
+                v[k] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
         }
-        __syncthreads();
+        float mine = v[0];
 #pragma unroll
-        for (int k = 0; k < K; k++) v[k] = warp_sum(lane < W ? b[k * W + lane] : 0.f);
+        for (int o = LANES / 2; o > 0; o /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        const int k = lane / LANES, sub = lane % LANES;                // mine: the warp's sum of value k
+        if (W > 1) {
+            float *b = buf + flip * (K * W);
+            flip ^= 1;
+            if (sub == 0) b[k * W + w] = mine;
+            __syncthreads();
+            mine = 0.f;
+#pragma unroll
+            for (int i = 0; i < (W + LANES - 1) / LANES; i++) { const int j = i * LANES + sub; mine += j < W ? b[k * W + j] : 0.f; }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o /= 2) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        }
+#pragma unroll
+        for (int i = 0; i < K; i++) v[i] = __shfl_sync(0xffffffffu, mine, i * LANES);
     }
 };
 
@@ -59,6 +77,16 @@ struct Piece {
 #pragma unroll
             for (int i = 0; i < NV * 4; i++) v[i] = p && has(i) ? p[at(i)] : missing;
         }
+    }
+    // the same values on their way into a place of shared memory that only this thread reads
+    __device__ __forceinline__ void ask(float *to, const float *p) const {
+        const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
+#pragma unroll
+        for (int i = 0; i < NV * 4; i += VEC ? 4 : 1)
+            if (has(i)) {
+                if (VEC) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + at(i) * 4), "l"(p + at(i)) : "memory");
+                else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + at(i) * 4), "l"(p + at(i)) : "memory");
+            }
     }
     __device__ __forceinline__ void store(float *p, const float (&v)[NV * 4]) const {
         if (VEC) {
@@ -160,7 +188,7 @@ struct BwdArgs {
     float *df, *dr;
     float *param_part, *gate_part;          // [block][4][cols] of dg2, db2, dg1, db1; [unit][cols] of dgate, which is dgate itself where a unit is a group
     float res_scale;
-    int cols, rows, layer, post, inc_df, inc_dr;         // inc: 0 store, 1 add, 2 add to a destination known to hold zeros
+    int cols, chunk, rows, layer, post, inc_df, inc_dr; // chunk: columns of one block of a cluster;         // inc: 0 store, 1 add, 2 add to a destination known to hold zeros
     int want_gate, want_param, inc_gate;    // want_param: bits dg2, db2, dg1, db1; inc_gate: add to gate_part
     int unit_groups, slices, workers;       // a unit is a slice of a group's rows; workers: blocks (clusters) that share the units
     size_t unit_rows;                       // rows of one unit group
@@ -175,64 +203,80 @@ struct BwdArgs {
 //     <dn1 n1> = <G e n1> - rstd2 (<dn2> <G n1> + <dn2 n2> <G n2 n1>)
 // and a row takes one exchange between its threads instead of two.  The column sums stay in registers over all rows of a block
 // and are added in a fixed order afterwards: no atomics.
+//
+// A row's four tensors are copied (cp.async) while the row before it is worked on, each value into a place that only the thread that
+// uses it reads, so the copies need no barrier; GENERAL: with means or shifts, eight sums a row, else three.
 template <int TPR, int NV, bool VEC, bool GENERAL, bool CLUSTER>
 __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kernel(const BwdArgs a) {
+    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4, K = GENERAL ? 8 : 4, SPAN = TPR * N;
+    extern __shared__ __align__(16) float staged[];                    // [team][2][dh, dr_out, r_out, f][SPAN]; at a unit's end the column sums of the teams
+    __shared__ __align__(16) float sums[2 * K * (TPR / 32)];
+    __shared__ __align__(16) float peers[CLUSTER ? 2 * K * 4 : 4];
     EB_GRID_WAIT();
-    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4, K = GENERAL ? 8 : 3;
-    extern __shared__ float team_sums[];                               // TPR == 32: the column sums of the block's teams, one kind at a time
-    __shared__ float sums[2 * K * (TPR / 32)];
-    __shared__ float peers[CLUSTER ? 2 * K * 4 : 1];
     TeamSum<TPR, K> sum(sums);
     const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0, csize = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
-    const int worker = (int)(blockIdx.x / csize), col0 = rank * (TPR * N), cols_here = min(a.cols - col0, TPR * N);
+    const int worker = (int)(blockIdx.x / csize), col0 = rank * a.chunk, cols_here = max(0, min(a.cols - col0, a.chunk));
     const Piece<TPR, NV, VEC> piece{(int)(threadIdx.x % TPR), cols_here};
     const int team = threadIdx.x / TPR;
+    float *own = staged + (size_t)team * (8 * SPAN);
     const float inv = 1.f / (float)a.cols;
-    int flip = 0;
-    float g2[N], gg[N], acc[GENERAL ? 4 : 2][N] = {}, acc_gate[N] = {};
+    int flip = 0, stage = 0;
+    float g2[N], g1[N], gate[N], acc[GENERAL ? 4 : 2][N] = {}, acc_gate[N] = {};
     piece.load(g2, a.g2 ? a.g2 + col0 : nullptr, a.g2 ? 0.f : 1.f);
+    piece.load(g1, a.g1 ? a.g1 + col0 : nullptr, a.g1 ? 0.f : 1.f);
+    piece.load(gate, nullptr, 1.f);
     if (!a.dh) {
 #pragma unroll
         for (int i = 0; i < N; i++) g2[i] = 0.f;
     }
+    float4 next_stats = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto ask = [&](size_t row, int to) {
+        const size_t base = row * a.cols + col0;
+        float *slot = own + to * (4 * SPAN);
+        if (a.dh) { piece.ask(slot, a.dh + base); piece.ask(slot + 2 * SPAN, a.r_out + base); }
+        if (a.dr_out) piece.ask(slot + SPAN, a.dr_out + base);
+        if (a.f) piece.ask(slot + 3 * SPAN, a.f + base);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next_stats = *reinterpret_cast<const float4 *>(a.stats + row * 4);
+    };
     const int units = a.unit_groups * a.slices;
+    size_t gate_of = ~(size_t)0;
     for (int unit = worker; unit < units; unit += a.workers) {
         const size_t group = unit / a.slices, slice = unit % a.slices;
         const size_t first = group * a.unit_rows + a.unit_rows * slice / a.slices, last = group * a.unit_rows + a.unit_rows * (slice + 1) / a.slices;
-        for (size_t row = first + team; row < last; row += TEAMS) {
+        if (first + team < last) ask(first + team, stage);
+        for (size_t row = first + team; row < last; row += TEAMS, stage ^= 1) {
             const size_t base = row * a.cols + col0;
-            const float4 st = *reinterpret_cast<const float4 *>(a.stats + row * 4);
-            float dh[N], e[N], n1[N], n2[N], gate[N];
-            piece.load(dh, a.dh ? a.dh + base : nullptr, 0.f);
-            piece.load(e, a.dr_out ? a.dr_out + base : nullptr, 0.f);
-            piece.load(n2, a.dh ? a.r_out + base : nullptr, 0.f);
-            piece.load(n1, a.f ? a.f + base : nullptr, 0.f);
-            piece.load(gate, a.gate ? a.gate + row / a.rows * a.cols + col0 : nullptr, 1.f);
-            if (a.g1) {
-                piece.load(gg, a.g1 + col0, 0.f);
-#pragma unroll
-                for (int i = 0; i < N; i++) gg[i] *= gate[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; i++) gg[i] = gate[i];
-            }
+            const float4 st = next_stats;
+            if (row + TEAMS < last) {
+                ask(row + TEAMS, stage ^ 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else asm volatile("cp.async.wait_group 0;" ::: "memory");
+            const float *slot = own + stage * (4 * SPAN);
+            if (a.gate && row / a.rows != gate_of) { gate_of = row / a.rows; piece.load(gate, a.gate + gate_of * a.cols + col0, 0.f); }
+            float dh[N], e[N], n1[N], n2[N];
+            piece.load(dh, a.dh ? slot : nullptr, 0.f);
+            piece.load(n2, a.dh ? slot + 2 * SPAN : nullptr, 0.f);
+            piece.load(e, a.dr_out ? slot + SPAN : nullptr, 0.f);
+            piece.load(n1, a.f ? slot + 3 * SPAN : nullptr, 0.f);
             float s[K] = {};
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                if (!piece.has(i)) { n1[i] = n2[i] = 0.f; gg[i] = 0.f; continue; }
+                if (!piece.has(i)) { n1[i] = n2[i] = 0.f; continue; }
+                const float gg = gate[i] * g1[i];
                 n2[i] = (n2[i] - st.z) * st.w;
                 if (a.post) n1[i] = (n1[i] - st.x) * st.y;
                 const float dn2 = dh[i] * g2[i];
                 e[i] += st.w * dn2;
                 s[0] += dn2 * n2[i];
-                s[1] += gg[i] * e[i] * n1[i];
-                s[2] += gg[i] * n2[i] * n1[i];
+                s[1] += gg * e[i] * n1[i];
+                s[2] += gg * n2[i] * n1[i];
                 if (GENERAL) {
-                    s[3] += dn2;
-                    s[4] += gg[i] * e[i];
-                    s[5] += gg[i];
-                    s[6] += gg[i] * n2[i];
-                    s[7] += gg[i] * n1[i];
+                    s[3 % K] += dn2;
+                    s[4 % K] += gg * e[i];
+                    s[5 % K] += gg;
+                    s[6 % K] += gg * n2[i];
+                    s[7 % K] += gg * n1[i];
                 }
             }
             sum(s);
@@ -241,29 +285,29 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
                 float *mine = peers + flip * (K * 4);
                 flip ^= 1;
                 if (threadIdx.x < (unsigned)csize) {
-                    float *there = cl.map_shared_rank(mine, threadIdx.x);
+                    float4 *there = reinterpret_cast<float4 *>(cl.map_shared_rank(mine, threadIdx.x) + rank * K);
 #pragma unroll
-                    for (int k = 0; k < K; k++) there[k * 4 + rank] = s[k];
+                    for (int k = 0; k < K; k += 4) there[k / 4] = make_float4(s[k], s[k + 1], s[k + 2], s[k + 3]);
                 }
                 cl.sync();
 #pragma unroll
-                for (int k = 0; k < K; k++) {
-                    s[k] = 0.f;
-                    for (int c = 0; c < csize; c++) s[k] += mine[k * 4 + c];
-                }
+                for (int k = 0; k < K; k++) s[k] = 0.f;
+                for (int c = 0; c < csize; c++)
+#pragma unroll
+                    for (int k = 0; k < K; k++) s[k] += mine[c * K + k];
             }
-            const float m_n2 = s[0] * inv, m_1 = GENERAL && a.layer ? s[3] * inv : 0.f;
-            const float q_n1 = s[1] * inv - st.w * (m_n2 * (s[2] * inv) + (GENERAL ? m_1 * (s[7] * inv) : 0.f));
-            const float q_1 = GENERAL && a.layer ? s[4] * inv - st.w * (m_n2 * (s[6] * inv) + m_1 * (s[5] * inv)) : 0.f;
+            const float m_n2 = s[0] * inv, m_1 = GENERAL && a.layer ? s[3 % K] * inv : 0.f;
+            const float q_n1 = s[1] * inv - st.w * (m_n2 * (s[2] * inv) + (GENERAL ? m_1 * (s[7 % K] * inv) : 0.f));
+            const float q_1 = GENERAL && a.layer ? s[4 % K] * inv - st.w * (m_n2 * (s[6 % K] * inv) + m_1 * (s[5 % K] * inv)) : 0.f;
             float out[N];
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float u = e[i] - st.w * (m_1 + n2[i] * m_n2);
+                const float u = e[i] - st.w * (m_1 + n2[i] * m_n2), du = gate[i] * u;
                 acc[0][i] += dh[i] * n2[i];
-                acc[1][i] += gate[i] * u * n1[i];
-                if (GENERAL) { acc[2][i] += dh[i]; acc[3][i] += gate[i] * u; }
+                acc[1][i] += du * n1[i];
+                if (GENERAL) { acc[2 % (GENERAL ? 4 : 2)][i] += dh[i]; acc[3 % (GENERAL ? 4 : 2)][i] += du; }
                 e[i] = u;
-                const float dn1 = gg[i] * u;
+                const float dn1 = du * g1[i];
                 out[i] = a.post ? st.y * (dn1 - q_1 - n1[i] * q_n1) : dn1;
             }
             if (a.df) {
@@ -276,11 +320,15 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
                 piece.store(a.df + base, out);
             }
             if (a.want_gate) {
-                float p[N], b[N];
-                piece.load(p, a.g1 ? a.g1 + col0 : nullptr, 1.f);
-                piece.load(b, a.b1 ? a.b1 + col0 : nullptr, 0.f);
+                if (a.b1) {
+                    float b[N];
+                    piece.load(b, a.b1 + col0, 0.f);
 #pragma unroll
-                for (int i = 0; i < N; i++) acc_gate[i] += e[i] * (n1[i] * p[i] + b[i]);
+                    for (int i = 0; i < N; i++) acc_gate[i] += e[i] * (n1[i] * g1[i] + b[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; i++) acc_gate[i] += e[i] * (n1[i] * g1[i]);
+                }
             }
             if (a.dr) {
                 if (a.inc_dr) {
@@ -305,14 +353,15 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
                 }
                 piece.store(dst, acc_gate);
             } else {
-                __syncthreads();
-                piece.store(team_sums + team * a.cols, acc_gate);
+                __syncthreads();                               // no copy is on its way, and no team still reads its places
+                piece.store(staged + team * a.cols, acc_gate);
                 __syncthreads();
                 for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
                     float t = 0.f;
-                    for (int k = 0; k < TEAMS; k++) t += team_sums[k * a.cols + c];
+                    for (int k = 0; k < TEAMS; k++) t += staged[k * a.cols + c];
                     dst[c] = a.inc_gate ? dst[c] + t : t;
                 }
+                __syncthreads();
             }
 #pragma unroll
             for (int i = 0; i < N; i++) acc_gate[i] = 0.f;
@@ -328,11 +377,11 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
         if (TEAMS == 1) piece.store(dst, acc[GENERAL ? which : which & 1]);
         else {
             __syncthreads();
-            piece.store(team_sums + team * a.cols, acc[GENERAL ? which : which & 1]);
+            piece.store(staged + team * a.cols, acc[GENERAL ? which : which & 1]);
             __syncthreads();
             for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
                 float t = 0.f;
-                for (int k = 0; k < TEAMS; k++) t += team_sums[k * a.cols + c];
+                for (int k = 0; k < TEAMS; k++) t += staged[k * a.cols + c];
                 dst[c] = t;
             }
         }
@@ -340,34 +389,37 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
     if (CLUSTER) cg::this_cluster().sync();                 // a block's slots outlive the writes of the others
 }
 
-// Column sums of the partial rows, in a fixed order: y 0..3 the parameters' gradients, from 4 on dgate of group y - 4.
+// Column sums of the partial rows, in a fixed order: the parameters' gradients over the blocks, dgate over a group's slices.  A block of 32 columns x 32
+// rows of threads gives every output as many rows of threads as it has partial rows (a power of two up to 32) and the rest to further
+// outputs: 64 groups of six slices are 16 blocks of columns high, not 64.
 struct FoldArgs {
     const float *param_part, *gate_part;
     float *out[4], *dgate;
-    int cols, workers, slices, inc;
+    int cols, workers, slices, groups, inc;
+    int param_rows, gate_rows, param_blocks;               // rows of threads for an output (log2), blocks that the parameters take
 };
-constexpr int kFoldRows = 16;
-__global__ void __launch_bounds__(32 * kFoldRows) norm_residual_fold_kernel(const FoldArgs a) {
+__global__ void __launch_bounds__(1024) norm_residual_fold_kernel(const FoldArgs a) {
     EB_GRID_WAIT();
-    __shared__ float part[kFoldRows][33];
+    __shared__ float part[32][33];
     const int col = blockIdx.x * 32 + threadIdx.x;
-    const bool gate = blockIdx.y >= 4;
-    float *out = gate ? a.dgate + (size_t)(blockIdx.y - 4) * a.cols : a.out[blockIdx.y & 3];
-    if (!gate && !out) return;
-    const float *src = gate ? a.gate_part + (size_t)(blockIdx.y - 4) * a.slices * a.cols : a.param_part + (size_t)blockIdx.y * a.cols;
+    const bool gate = (int)blockIdx.y >= a.param_blocks;
+    const int log_rows = gate ? a.gate_rows : a.param_rows, row = threadIdx.y & ((1 << log_rows) - 1);
+    const int which = (((int)blockIdx.y - (gate ? a.param_blocks : 0)) << (5 - log_rows)) + (threadIdx.y >> log_rows);
+    const bool there = which < (gate ? a.groups : 4) && col < a.cols;
+    float *out = !there ? nullptr : gate ? a.dgate + (size_t)which * a.cols : which == 0 ? a.out[0] : which == 1 ? a.out[1] : which == 2 ? a.out[2] : a.out[3];
     const size_t step = gate ? a.cols : (size_t)4 * a.cols;
+    const float *src = gate ? a.gate_part + (size_t)which * a.slices * a.cols : a.param_part + (size_t)which * a.cols;
     const int n = gate ? a.slices : a.workers;
     float s = 0.f;
-    if (col < a.cols) {
-#pragma unroll 4
-        for (int i = threadIdx.y; i < n; i += kFoldRows) s += __ldcg(src + i * step + col);
+    if (out) {
+#pragma unroll 8
+        for (int i = row; i < n; i += 1 << log_rows) s += __ldcg(src + i * step + col);
     }
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y || col >= a.cols) return;
+    if (row || !out) return;
     float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < kFoldRows; i++) t += part[i][threadIdx.x];
+    for (int i = 0; i < 1 << log_rows; i++) t += part[threadIdx.y + i][threadIdx.x];
     out[col] = a.inc ? out[col] + t : t;
 }
 
@@ -380,13 +432,52 @@ void launch_fwd(cudaStream_t st, const FwdArgs &a, bool vec) {
 }
 
 template <int TPR, int NV, bool CLUSTER>
-void launch_bwd(cudaStream_t st, const BwdArgs &a, bool vec, bool general, unsigned csize) {
-    constexpr int block = TPR == 32 ? 256 : TPR;
-    const size_t smem = TPR == 32 ? (size_t)8 * a.cols * sizeof(float) : 0;
-    auto kernel = vec ? (general ? norm_residual_bwd_kernel<TPR, NV, true, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, true, false, CLUSTER>)
-                      : (general ? norm_residual_bwd_kernel<TPR, NV, false, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, false, false, CLUSTER>);
-    if (CLUSTER) eb::launch_cluster(kernel, csize, a.workers * csize, block, smem, st, a);
-    else eb::launch(kernel, a.workers, block, smem, st, a);
+struct Bwd {
+    static constexpr int block = TPR == 32 ? 256 : TPR, teams = TPR == 32 ? 8 : 1;
+    static constexpr size_t smem = (size_t)teams * 8 * TPR * NV * 4 * sizeof(float);
+    static auto kernel(bool vec, bool general) {
+        return vec ? (general ? norm_residual_bwd_kernel<TPR, NV, true, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, true, false, CLUSTER>)
+                   : (general ? norm_residual_bwd_kernel<TPR, NV, false, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, false, false, CLUSTER>);
+    }
+    // blocks (clusters of `csize`) that the device holds at once; 0 with the error set
+    static int resident(int dev, bool vec, bool general, unsigned csize) {
+        static int known[EDDLB200_MAX_DEVICES][4][5] = {};
+        int &n = known[dev][2 * vec + general][csize];
+        if (n) return n;
+        auto k = kernel(vec, general);
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        int held = 0;
+        if (e == cudaSuccess && CLUSTER) {
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension; at[0].val.clusterDim.x = csize; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+            cudaLaunchConfig_t c = {};
+            c.gridDim = dim3(EDDLB200_NUM_SMS / csize * csize); c.blockDim = dim3(block); c.dynamicSmemBytes = smem; c.attrs = at; c.numAttrs = 1;
+            e = cudaOccupancyMaxActiveClusters(&held, k, &c);
+        } else if (e == cudaSuccess) {
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, k, block, smem);
+            held *= EDDLB200_NUM_SMS;
+        }
+        if (e != cudaSuccess) { cuda_status(e, "norm_residual_bwd(occupancy)"); return 0; }
+        if (held < 1) { set_error(EDDLB200_ELIMIT, "norm_residual_bwd: the device holds no cluster of %u blocks", csize); return 0; }
+        return n = held;
+    }
+    static int launch(DevCtx *cx, cudaStream_t st, const BwdArgs &a, bool vec, bool general, unsigned csize) {
+        if (CLUSTER) eb::launch_cluster(kernel(vec, general), csize, a.workers * csize, block, smem, st, a);
+        else eb::launch(kernel(vec, general), a.workers, block, smem, st, a);
+        EB_LAUNCH_CHECK("norm_residual_bwd");
+        return 0;
+    }
+};
+// The smallest team that holds a row in registers beside its column sums: eight values a thread at most; wider rows are shared by a cluster.
+template <typename Go>
+auto with_bwd(int cols, Go go) {
+    if (cols <= 128) return go(Bwd<32, 1, false>());
+    if (cols <= 256) return go(Bwd<32, 2, false>());
+    if (cols <= 512) return go(Bwd<128, 1, false>());
+    if (cols <= 1024) return go(Bwd<128, 2, false>());
+    if (cols <= 2048) return go(Bwd<256, 2, false>());
+    if (cols <= 4096) return go(Bwd<512, 2, false>());
+    return go(Bwd<512, 2, true>());
 }
 
 // An output may be an input's own memory (every value is read before it is written, by the thread that writes it), but not part of it.
@@ -429,10 +520,11 @@ int eddlb200_norm_residual_fwd(int dev, int kind, int post, int groups, int rows
     ProfScope prof(cx, PROF_BN_FWD, (double)bytes * ((f ? 3 : 1) + (h ? 1 : 0)));
     const FwdArgs a{f, r, gate, g1, b1, g2, b2, r_out, h, stats, res_scale, eps, cols, rows, kind, post, total};
     const bool vec = cols % 4 == 0 && aligned16(f) && aligned16(r) && aligned16(gate) && aligned16(g1) && aligned16(b1) && aligned16(g2) && aligned16(b2) && aligned16(r_out) && aligned16(h);
+    const bool few = total < (size_t)EDDLB200_NUM_SMS * 8;          // rows for one warp a scheduler or less: several warps a row
     if (cols <= 128) launch_fwd<32, 1>(st, a, vec);
     else if (cols <= 256) launch_fwd<32, 2>(st, a, vec);
-    else if (cols <= 512) launch_fwd<128, 1>(st, a, vec);
-    else if (cols <= 1024) launch_fwd<128, 2>(st, a, vec);
+    else if (cols <= 512) { if (few) launch_fwd<128, 1>(st, a, vec); else launch_fwd<32, 4>(st, a, vec); }
+    else if (cols <= 1024) { if (few) launch_fwd<128, 2>(st, a, vec); else launch_fwd<32, 8>(st, a, vec); }
     else if (cols <= 2048) launch_fwd<256, 2>(st, a, vec);
     else if (cols <= 4096) launch_fwd<512, 2>(st, a, vec);
     else if (cols <= 8192) launch_fwd<1024, 2>(st, a, vec);
@@ -465,19 +557,27 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
         EB_REQUIRE(!(o < 2 && inc_d && out[o]) || (out[o] != dh && out[o] != dr_out && out[o] != f && out[o] != r_out), kBwd);
     }
     EB_CTX(dev);
-    const bool cluster = cols > 4096;
+    const bool cluster = cols > 4096, general = kind || db1 || db2;
     const unsigned csize = cluster ? (unsigned)ceil_div(cols, 4096) : 1;
-    const int team_rows = cols <= 256 ? 8 : 1, block = cols <= 256 ? 256 : cols <= 1024 ? 128 : cols <= 2048 ? 256 : 512;
-    BwdArgs a{dh, dr_out, f, r_out, gate, g1, b1, g2, stats, df, dr, nullptr, nullptr, res_scale, cols, rows, kind, post, 0, 0};
+    bool vec = cols % 4 == 0;
+    for (int i = 0; i < 8; i++) vec = vec && aligned16(in[i]);
+    vec = vec && aligned16(df) && aligned16(dr);
+    BwdArgs a{dh, dr_out, f, r_out, gate, g1, b1, g2, stats, df, dr, nullptr, nullptr, res_scale, cols, 0, rows, kind, post, 0, 0};
+    a.chunk = cluster ? (int)((ceil_div(cols, csize) + 3) & ~(size_t)3) : cols;
     a.want_gate = dgate != nullptr;
     a.want_param = (dg2 ? 1 : 0) | (db2 ? 2 : 0) | (dg1 ? 4 : 0) | (db1 ? 8 : 0);
     a.unit_groups = dgate ? groups : 1;
     a.unit_rows = dgate ? (size_t)rows : total;
-    const size_t most = (size_t)EDDLB200_NUM_SMS * (1024 / block) / csize, passes = total ? ceil_div(a.unit_rows, team_rows) : 1;
-    size_t slices = a.unit_groups ? ceil_div(most, a.unit_groups) : 1;
-    if (slices > passes) slices = passes;
-    if (slices < 1) slices = 1;
-    const size_t units = a.unit_groups * slices;
+    // slices of a group: so many that the rounds of units over the blocks take the fewest rows one after the other
+    const size_t most = total ? with_bwd(cols, [&](auto k) { return k.resident(dev, vec, general, csize); }) : 1;
+    if (!most) return EDDLB200_ELIMIT;
+    const size_t passes = total ? ceil_div(a.unit_rows, cols <= 256 ? 8 : 1) : 1;
+    size_t slices = 1, units = a.unit_groups, longest = ceil_div(units, most) * passes;
+    for (size_t rounds = 1; rounds <= 4 && a.unit_groups; rounds++) {
+        size_t s = rounds * most / a.unit_groups;
+        if (s > passes) s = passes;
+        if (s > 1 && rounds * ceil_div(passes, s) < longest) { slices = s; units = s * a.unit_groups; longest = rounds * ceil_div(passes, s); }
+    }
     a.slices = (int)slices;
     a.workers = (int)(units < most ? units : most);
     const size_t param_floats = a.want_param ? (size_t)a.workers * 4 * cols : 0, gate_floats = dgate && slices > 1 ? units * cols : 0;
@@ -513,22 +613,13 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
         return 0;
     }
     ProfScope prof(cx, PROF_BN_BWD, (double)bytes * ((dh ? 2 : 0) + (dr_out ? 1 : 0) + (f ? 1 : 0) + (df ? 1 + (inc[0] == 1) : 0) + (dr ? 1 + (inc[1] == 1) : 0)));
-    const bool general = kind || db1 || db2;
-    bool vec = cols % 4 == 0;
-    for (int i = 0; i < 8; i++) vec = vec && aligned16(in[i]);
-    vec = vec && aligned16(df) && aligned16(dr);
-    if (cols <= 128) launch_bwd<32, 1, false>(st, a, vec, general, 1);
-    else if (cols <= 256) launch_bwd<32, 2, false>(st, a, vec, general, 1);
-    else if (cols <= 512) launch_bwd<128, 1, false>(st, a, vec, general, 1);
-    else if (cols <= 1024) launch_bwd<128, 2, false>(st, a, vec, general, 1);
-    else if (cols <= 2048) launch_bwd<256, 2, false>(st, a, vec, general, 1);
-    else if (cols <= 4096) launch_bwd<512, 2, false>(st, a, vec, general, 1);
-    else launch_bwd<512, 2, true>(st, a, vec, general, csize);
-    EB_LAUNCH_CHECK(kBwd);
+    if (int e = with_bwd(cols, [&](auto k) { return k.launch(cx, st, a, vec, general, csize); })) return e;
     if (!fold) return 0;
-    const FoldArgs fa{a.param_part, a.gate_part, {dg2, db2, dg1, db1}, dgate, cols, a.workers, a.slices, inc_g};
-    const unsigned kinds = 4 + (gate_floats ? (unsigned)groups : 0);           // fewer groups than units that run at a time, so far below the grid's limit
-    eb::launch(norm_residual_fold_kernel, dim3((unsigned)ceil_div(cols, 32), kinds), dim3(32, kFoldRows), 0, st, fa);
+    auto log_rows = [](int n) { int l = 0; while (l < 5 && (1 << l) < n) l++; return l; };
+    FoldArgs fa{a.param_part, a.gate_part, {dg2, db2, dg1, db1}, dgate, cols, a.workers, a.slices, gate_floats ? groups : 0, inc_g, log_rows(a.workers), log_rows(a.slices), 0};
+    fa.param_blocks = a.want_param ? (int)ceil_div(4, (size_t)32 >> fa.param_rows) : 0;
+    const size_t gate_blocks = ceil_div((size_t)fa.groups, (size_t)32 >> fa.gate_rows);         // fewer groups than blocks that run at a time: far below the grid's limit
+    eb::launch(norm_residual_fold_kernel, dim3((unsigned)ceil_div(cols, 32), (unsigned)(fa.param_blocks + gate_blocks)), dim3(32, 32), 0, st, fa);
     EB_LAUNCH_CHECK(kBwd);
     return 0;
 }
