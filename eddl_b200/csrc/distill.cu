@@ -468,9 +468,10 @@ extern "C" int eddlb200_distill(int dev, const float *logits, const int *ids, co
                                 const float *weights, int rows, int cols, size_t ld, int k, float temperature, float alpha, float *loss, float *delta) {
     const char *what = "distill";
     EB_REQUIRE(rows >= 0 && cols > 0 && k > 0 && ld >= (size_t)cols, what);
-    EB_REQUIRE(temperature > 0.f && temperature < INFINITY, what);
+    EB_REQUIRE(temperature >= 1.17549435e-38f && temperature < INFINITY, what);
     EB_REQUIRE(alpha >= 0.f && alpha <= 1.f, what);
     if (cols > kMaxCols) return set_error(EDDLB200_ELIMIT, "%s: %d classes, at most %d", what, cols, kMaxCols);
+    if (rows > 0x7fff0000) return set_error(EDDLB200_ELIMIT, "%s: %d rows", what, rows);
     if (k > kMaxTop) return set_error(EDDLB200_ELIMIT, "%s: %d entries a row, at most %d", what, k, kMaxTop);
     EB_REQUIRE(!rows || (logits && ids && teacher && loss), what);
     EB_REQUIRE(!rows || labels || alpha == 0.f, what);

@@ -9,6 +9,7 @@ namespace {
 using namespace eb;
 
 constexpr int kBlk = 128;
+constexpr int kMaxSide = 0x7fffff00;            // indexes within the last tile of a side stay in 32 bits
 
 // ---- quantisation ------------------------------------------------------------------------------------------------------------
 // One block per 128 x 128 tile, one read of it for both directions; bound by memory (4 bytes read, 1 or 2 written a value).  A warp
@@ -709,7 +710,7 @@ int eddlb200_fp8_quantize(int dev, const float *a, int rows, int cols, int forma
     EB_REQUIRE(!qt || (scale_t && aligned16(qt) && ldqt % 16 == 0 && ldqt >= (size_t)rows), what);
     EB_REQUIRE(!rows || !cols || a, what);
     const size_t tiles = ceil_div(rows, kBlk) * ceil_div(cols, kBlk);
-    if (tiles > 0x7fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, rows, cols);
+    if (rows > kMaxSide || cols > kMaxSide || tiles > 0x7fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, rows, cols);
     const size_t in = (size_t)rows * cols * sizeof(float);
     const void *out[] = {q, scale, qt, scale_t};
     const size_t bytes[] = {matrix_bytes(rows, cols, ldq), scale_bytes(rows, cols, block_rows), matrix_bytes(cols, rows, ldqt), scale_bytes(cols, rows, block_rows)};
@@ -744,7 +745,7 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     EB_REQUIRE(lda < ((size_t)1 << 40) && ldb < ((size_t)1 << 40), what);
     EB_REQUIRE(!m || !n || c, what);
     EB_REQUIRE(!m || !n || !k || (qa && qb && scale_a && scale_b && aligned16(qa) && aligned16(qb)), what);
-    if (k > 0x7fffff00) return set_error(EDDLB200_ELIMIT, "%s: k = %d", what, k);
+    if (m > kMaxSide || n > kMaxSide || k > kMaxSide) return set_error(EDDLB200_ELIMIT, "%s: %d x %d x %d", what, m, n, k);
     const size_t out = (size_t)m * n * sizeof(float);
     const void *in[] = {qa, qb, scale_a, scale_b};
     const size_t bytes[] = {matrix_bytes(m, k, lda), matrix_bytes(n, k, ldb), scale_bytes(m, k, block_a), scale_bytes(n, k, block_b)};

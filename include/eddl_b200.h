@@ -130,7 +130,7 @@ int eddlb200_accuracy(int dev, const float *y_true, const float *y_pred, int row
 
 /* Distillation (no counterpart in EDDL): loss of a student's logits [rows, cols] (rows `ld` floats apart, like delta's; at most 344064 columns)
  * against the teacher's k <= 1024 best classes of each row -- ids [rows, k] and teacher [rows, k], the teacher's logits -- mixed with the
- * cross-entropy of hard labels [rows], and its gradient.  With x a row, q = softmax(x / T), T = temperature:
+ * cross-entropy of hard labels [rows], and its gradient.  With x a row, q = softmax(x / T), T = temperature (a normal number above 0):
  *   loss[row] = w ((1 - alpha) T^2 KL + alpha (log sum exp x - x_label)),   delta = d loss[row] / d x
  *   teacher_lse null:  KL = sum_j p_j log(p_j / q_j),  p = softmax of teacher / T over the row's entries
  *   else [rows], log sum exp(t / T) over ALL of the teacher's classes:  p_j = exp(teacher_j / T - teacher_lse), and p_r = max(0, 1 - sum p_j), the

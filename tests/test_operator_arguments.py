@@ -10,7 +10,7 @@ P = [0x10000000 * (i + 1) for i in range(24)]          # addresses far apart tha
 
 
 def call(name, args):
-    conv = [ctypes.c_void_p(a) if isinstance(a, int) and a in P else a for a in args]
+    conv = [ctypes.c_void_p(a) if isinstance(a, int) and (a in P or a >= 1 << 50) else a for a in args]
     return capi.lib().fn[name](*conv)
 
 
@@ -76,7 +76,7 @@ DIST_OK = [0, P[0], P[1], P[2], P[3], P[4], P[5], 6, 100, 104, 5, 2.0, 0.5, P[6]
 
 
 @pytest.mark.parametrize("change", [
-    dict(logits=None), dict(ids=None), dict(teacher=None), dict(loss=None), dict(labels=None), dict(rows=-1), dict(cols=0), dict(ld=99), dict(k=0), dict(k=-1), dict(temperature=0.0), dict(temperature=-1.0),
+    dict(logits=None), dict(ids=None), dict(teacher=None), dict(loss=None), dict(labels=None), dict(rows=-1), dict(cols=0), dict(ld=99), dict(k=0), dict(k=-1), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=1e-39),
     dict(temperature=float("inf")), dict(temperature=float("nan")), dict(alpha=-0.1), dict(alpha=1.1), dict(alpha=float("nan")), dict(delta=P[0] + 4), dict(delta=P[1]), dict(loss=P[0]), dict(loss=P[7]), dict(loss=P[5])])
 def test_distill_refuses(change):
     assert call("distill", with_changes(DIST, DIST_OK, change)) == INVAL
@@ -88,6 +88,9 @@ def test_limits_are_told_apart_from_mistakes():
     assert call("norm_residual_bwd", with_changes(BWD, BWD_OK, dict(cols=16385))) == LIMIT
     assert call("distill", with_changes(DIST, DIST_OK, dict(cols=344065, ld=344065))) == LIMIT
     assert call("distill", with_changes(DIST, DIST_OK, dict(k=1025))) == LIMIT
+    assert call("distill", with_changes(DIST, DIST_OK, dict(rows=2 ** 31 - 1, delta=None, loss=1 << 60))) == LIMIT
+    assert call("fp8_quantize", with_changes(QUANT, QUANT_OK, dict(rows=1, cols=2 ** 31 - 1, ldq=(1 << 31) + 16, qt=None, q=1 << 60, scale=1 << 61))) == LIMIT
+    assert call("fp8_mult2d", with_changes(PROD, PROD_OK, dict(m=2 ** 31 - 1, c=1 << 60, qb=1 << 61, sb=1 << 62, sa=3 << 60))) == LIMIT
 
 
 def test_right_arguments_reach_the_device():
