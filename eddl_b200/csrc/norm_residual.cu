@@ -14,7 +14,8 @@ namespace {
 using namespace eb;
 namespace cg = cooperative_groups;
 
-constexpr int kMaxCols = 16384;            // 1024 threads with four 16-byte pieces each; four blocks of 512 with two each
+constexpr int kMaxCols = 16384;            // 1024 threads with four 16-byte pieces each; eight blocks of 256 with two each
+constexpr int kMaxCluster = 8;
 
 // Sums of K values over a team of TPR threads (a warp, or the whole block); every thread gets them, added in a fixed order.  K is a power of two:
 // the lanes halve the number of values they carry with each of the first exchanges, so K sums of a warp cost K + 1 shuffles or so, not 5 K.
@@ -78,15 +79,28 @@ struct Piece {
             for (int i = 0; i < NV * 4; i++) v[i] = p && has(i) ? p[at(i)] : missing;
         }
     }
-    // the same values on their way into a place of shared memory that only this thread reads
+    // a row of them on its way into shared memory: value c comes to lie at to[misfit(p) + c].  own(): every thread copies what it will read itself (the
+    // rows of a warp, few values each, 4 bytes at a time where they are not aligned); else 16 bytes at a time, the team's threads for one another
+    static constexpr __device__ __forceinline__ bool own() { return VEC || TPR == 32; }
+    static __device__ __forceinline__ int misfit(const float *p) { return own() ? 0 : (int)((uintptr_t)p >> 2) & 3; }
     __device__ __forceinline__ void ask(float *to, const float *p) const {
         const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
+        if (!VEC && own()) {
 #pragma unroll
-        for (int i = 0; i < NV * 4; i += VEC ? 4 : 1)
-            if (has(i)) {
-                if (VEC) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + at(i) * 4), "l"(p + at(i)) : "memory");
-                else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + at(i) * 4), "l"(p + at(i)) : "memory");
+            for (int i = 0; i < NV * 4; i++) if (has(i)) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + at(i) * 4), "l"(p + at(i)) : "memory");
+            return;
+        }
+        const int off = misfit(p), end = off + cols;
+#pragma unroll
+        for (int k = 0; k < NV + (VEC ? 0 : 1); k++) {
+            const int u = (k * TPR + t) * 4;
+            if (u >= off && u + 4 <= end) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + u * 4), "l"(p - off + u) : "memory");
+            else if (!VEC && u < end) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (u + i >= off && u + i < end) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + (u + i) * 4), "l"(p - off + u + i) : "memory");
             }
+        }
     }
     __device__ __forceinline__ void store(float *p, const float (&v)[NV * 4]) const {
         if (VEC) {
@@ -183,6 +197,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_fwd_kerne
     }
 }
 
+constexpr int BWD_THREADS = 512;          // of an SM: 128 registers each
 struct BwdArgs {
     const float *dh, *dr_out, *f, *r_out, *gate, *g1, *b1, *g2, *stats;
     float *df, *dr;
@@ -204,14 +219,15 @@ struct BwdArgs {
 // and a row takes one exchange between its threads instead of two.  The column sums stay in registers over all rows of a block
 // and are added in a fixed order afterwards: no atomics.
 //
-// A row's four tensors are copied (cp.async) while the row before it is worked on, each value into a place that only the thread that
-// uses it reads, so the copies need no barrier; GENERAL: with means or shifts, eight sums a row, else three.
+// A row's four tensors are copied (cp.async, 16 bytes) while the row before it is worked on.  VEC: 16-byte aligned rows, each value comes to a place
+// that only the thread that uses it reads, so the copies need no barrier; else a barrier a row (with 4-byte copies by the thread
+// itself 38 x 555 x 1551 took 487 us, forward and backward).  GENERAL: with means or shifts, eight sums a row, else three.
 template <int TPR, int NV, bool VEC, bool GENERAL, bool CLUSTER>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kernel(const BwdArgs a) {
-    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4, K = GENERAL ? 8 : 4, SPAN = TPR * N;
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, BWD_THREADS / (TPR == 32 ? 256 : TPR)) norm_residual_bwd_kernel(const BwdArgs a) {
+    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4, K = GENERAL ? 8 : 4, SPAN = TPR * N + (VEC ? 0 : 4);
     extern __shared__ __align__(16) float staged[];                    // [team][2][dh, dr_out, r_out, f][SPAN]; at a unit's end the column sums of the teams
     __shared__ __align__(16) float sums[2 * K * (TPR / 32)];
-    __shared__ __align__(16) float peers[CLUSTER ? 2 * K * 4 : 4];
+    __shared__ __align__(16) float peers[CLUSTER ? 2 * K * kMaxCluster : 4];
     EB_GRID_WAIT();
     TeamSum<TPR, K> sum(sums);
     const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0, csize = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
@@ -221,10 +237,38 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
     float *own = staged + (size_t)team * (8 * SPAN);
     const float inv = 1.f / (float)a.cols;
     int flip = 0, stage = 0;
-    float g2[N], g1[N], gate[N], acc[GENERAL ? 4 : 2][N] = {}, acc_gate[N] = {};
+    // Column sums: dg2, db2, and of u n1 and u over the rows of one gate, from which its dgate and its share of dg1 and db1 follow
+    float g2[N], gg[N], dg2[N] = {}, db2[GENERAL ? N : 1] = {}, un[N] = {}, uu[N] = {}, dg1[N] = {}, db1[GENERAL ? N : 1] = {}, gg_sum = 0.f;
+    size_t gate_of = 0;
     piece.load(g2, a.g2 ? a.g2 + col0 : nullptr, a.g2 ? 0.f : 1.f);
-    piece.load(g1, a.g1 ? a.g1 + col0 : nullptr, a.g1 ? 0.f : 1.f);
-    piece.load(gate, nullptr, 1.f);
+    auto gate_row = [&](float (&v)[N]) { piece.load(v, a.gate ? a.gate + gate_of * a.cols + col0 : nullptr, a.gate ? 0.f : 1.f); };
+    auto take_gate = [&](size_t which) {                       // gg = gate g1
+        gate_of = which;
+        float v[N];
+        gate_row(gg);
+        piece.load(v, a.g1 ? a.g1 + col0 : nullptr, a.g1 ? 0.f : 1.f);
+        gg_sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) { gg[i] = piece.has(i) ? gg[i] * v[i] : 0.f; gg_sum += gg[i]; }
+    };
+    auto settle = [&](float (&of_gate)[N]) {                   // the sums of this gate's rows go where they belong
+        float v[N];
+        gate_row(v);
+#pragma unroll
+        for (int i = 0; i < N; i++) { dg1[i] += v[i] * un[i]; if (GENERAL) db1[GENERAL ? i : 0] += v[i] * uu[i]; }
+        if (a.want_gate) {
+            piece.load(v, a.g1 ? a.g1 + col0 : nullptr, a.g1 ? 0.f : 1.f);
+#pragma unroll
+            for (int i = 0; i < N; i++) of_gate[i] = v[i] * un[i];
+            if (a.b1) {
+                piece.load(v, a.b1 + col0, 0.f);
+#pragma unroll
+                for (int i = 0; i < N; i++) of_gate[i] += v[i] * uu[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) un[i] = uu[i] = 0.f;
+    };
     if (!a.dh) {
 #pragma unroll
         for (int i = 0; i < N; i++) g2[i] = 0.f;
@@ -240,7 +284,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
         next_stats = *reinterpret_cast<const float4 *>(a.stats + row * 4);
     };
     const int units = a.unit_groups * a.slices;
-    size_t gate_of = ~(size_t)0;
+    bool started = false;
     for (int unit = worker; unit < units; unit += a.workers) {
         const size_t group = unit / a.slices, slice = unit % a.slices;
         const size_t first = group * a.unit_rows + a.unit_rows * slice / a.slices, last = group * a.unit_rows + a.unit_rows * (slice + 1) / a.slices;
@@ -253,36 +297,42 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
             } else asm volatile("cp.async.wait_group 0;" ::: "memory");
             const float *slot = own + stage * (4 * SPAN);
-            if (a.gate && row / a.rows != gate_of) { gate_of = row / a.rows; piece.load(gate, a.gate + gate_of * a.cols + col0, 0.f); }
+            if (!started) { take_gate(a.gate ? row / a.rows : 0); started = true; }
+            else if (a.gate && row / a.rows != gate_of) {
+                float unused[N];
+                if (!a.want_gate) settle(unused);
+                take_gate(row / a.rows);
+            }
+            // where the threads copy for one another: a place is copied into again only after the barrier of this row's sums
+            if (!piece.own()) __syncthreads();
             float dh[N], e[N], n1[N], n2[N];
-            piece.load(dh, a.dh ? slot : nullptr, 0.f);
-            piece.load(n2, a.dh ? slot + 2 * SPAN : nullptr, 0.f);
-            piece.load(e, a.dr_out ? slot + SPAN : nullptr, 0.f);
-            piece.load(n1, a.f ? slot + 3 * SPAN : nullptr, 0.f);
+            piece.load(dh, a.dh ? slot + piece.misfit(a.dh + base) : nullptr, 0.f);
+            piece.load(n2, a.dh ? slot + 2 * SPAN + piece.misfit(a.r_out + base) : nullptr, 0.f);
+            piece.load(e, a.dr_out ? slot + SPAN + piece.misfit(a.dr_out + base) : nullptr, 0.f);
+            piece.load(n1, a.f ? slot + 3 * SPAN + piece.misfit(a.f + base) : nullptr, 0.f);
             float s[K] = {};
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 if (!piece.has(i)) { n1[i] = n2[i] = 0.f; continue; }
-                const float gg = gate[i] * g1[i];
                 n2[i] = (n2[i] - st.z) * st.w;
                 if (a.post) n1[i] = (n1[i] - st.x) * st.y;
-                const float dn2 = dh[i] * g2[i];
+                const float dn2 = dh[i] * g2[i], gn = gg[i] * n1[i];
                 e[i] += st.w * dn2;
                 s[0] += dn2 * n2[i];
-                s[1] += gg * e[i] * n1[i];
-                s[2] += gg * n2[i] * n1[i];
+                s[1] += gn * e[i];
+                s[2] += gn * n2[i];
                 if (GENERAL) {
                     s[3 % K] += dn2;
-                    s[4 % K] += gg * e[i];
-                    s[5 % K] += gg;
-                    s[6 % K] += gg * n2[i];
-                    s[7 % K] += gg * n1[i];
+                    s[4 % K] += gg[i] * e[i];
+                    s[6 % K] += gg[i] * n2[i];
+                    s[7 % K] += gn;
                 }
             }
+            if (GENERAL) s[5 % K] = gg_sum;
             sum(s);
             if (CLUSTER) {
                 cg::cluster_group cl = cg::this_cluster();
-                float *mine = peers + flip * (K * 4);
+                float *mine = peers + flip * (K * kMaxCluster);
                 flip ^= 1;
                 if (threadIdx.x < (unsigned)csize) {
                     float4 *there = reinterpret_cast<float4 *>(cl.map_shared_rank(mine, threadIdx.x) + rank * K);
@@ -302,12 +352,12 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
             float out[N];
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float u = e[i] - st.w * (m_1 + n2[i] * m_n2), du = gate[i] * u;
-                acc[0][i] += dh[i] * n2[i];
-                acc[1][i] += du * n1[i];
-                if (GENERAL) { acc[2 % (GENERAL ? 4 : 2)][i] += dh[i]; acc[3 % (GENERAL ? 4 : 2)][i] += du; }
+                const float u = e[i] - st.w * (m_1 + n2[i] * m_n2);
+                dg2[i] += dh[i] * n2[i];
+                un[i] += u * n1[i];
+                if (GENERAL) { db2[GENERAL ? i : 0] += dh[i]; uu[i] += u; }
                 e[i] = u;
-                const float dn1 = du * g1[i];
+                const float dn1 = u * gg[i];
                 out[i] = a.post ? st.y * (dn1 - q_1 - n1[i] * q_n1) : dn1;
             }
             if (a.df) {
@@ -318,17 +368,6 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
                     for (int i = 0; i < N; i++) out[i] += old[i];
                 }
                 piece.store(a.df + base, out);
-            }
-            if (a.want_gate) {
-                if (a.b1) {
-                    float b[N];
-                    piece.load(b, a.b1 + col0, 0.f);
-#pragma unroll
-                    for (int i = 0; i < N; i++) acc_gate[i] += e[i] * (n1[i] * g1[i] + b[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; i++) acc_gate[i] += e[i] * (n1[i] * g1[i]);
-                }
             }
             if (a.dr) {
                 if (a.inc_dr) {
@@ -343,18 +382,20 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
             }
         }
         if (a.want_gate) {
+            float of_gate[N] = {};
+            if (started) settle(of_gate);
             float *dst = a.gate_part + (size_t)unit * a.cols + col0;
             if (TEAMS == 1) {
                 if (a.inc_gate) {
                     float old[N];
                     piece.load(old, dst, 0.f);
 #pragma unroll
-                    for (int i = 0; i < N; i++) acc_gate[i] += old[i];
+                    for (int i = 0; i < N; i++) of_gate[i] += old[i];
                 }
-                piece.store(dst, acc_gate);
+                piece.store(dst, of_gate);
             } else {
                 __syncthreads();                               // no copy is on its way, and no team still reads its places
-                piece.store(staged + team * a.cols, acc_gate);
+                piece.store(staged + team * a.cols, of_gate);
                 __syncthreads();
                 for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
                     float t = 0.f;
@@ -363,29 +404,25 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_bwd_kerne
                 }
                 __syncthreads();
             }
-#pragma unroll
-            for (int i = 0; i < N; i++) acc_gate[i] = 0.f;
         }
     }
+    if (!a.want_gate && started) { float unused[N]; settle(unused); }
     // kinds in the order of param_part: dg2, db2, dg1, db1
-#pragma unroll
-    for (int kind = 0; kind < 4; kind++) {
-        if (!(a.want_param >> kind & 1)) continue;
-        const int which = kind == 0 ? 0 : kind == 1 ? 2 : kind == 2 ? 1 : 3;
-        if (!GENERAL && which >= 2) continue;
+    auto leave = [&](int kind, const float (&v)[N]) {
+        if (!(a.want_param >> kind & 1)) return;
         float *dst = a.param_part + ((size_t)worker * 4 + kind) * a.cols + col0;
-        if (TEAMS == 1) piece.store(dst, acc[GENERAL ? which : which & 1]);
-        else {
-            __syncthreads();
-            piece.store(staged + team * a.cols, acc[GENERAL ? which : which & 1]);
-            __syncthreads();
-            for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
-                float t = 0.f;
-                for (int k = 0; k < TEAMS; k++) t += staged[k * a.cols + c];
-                dst[c] = t;
-            }
+        if (TEAMS == 1) { piece.store(dst, v); return; }
+        __syncthreads();
+        piece.store(staged + team * a.cols, v);
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+            float t = 0.f;
+            for (int k = 0; k < TEAMS; k++) t += staged[k * a.cols + c];
+            dst[c] = t;
         }
-    }
+    };
+    leave(0, dg2); leave(2, dg1);
+    if constexpr (GENERAL) { leave(1, db2); leave(3, db1); }
     if (CLUSTER) cg::this_cluster().sync();                 // a block's slots outlive the writes of the others
 }
 
@@ -434,14 +471,14 @@ void launch_fwd(cudaStream_t st, const FwdArgs &a, bool vec) {
 template <int TPR, int NV, bool CLUSTER>
 struct Bwd {
     static constexpr int block = TPR == 32 ? 256 : TPR, teams = TPR == 32 ? 8 : 1;
-    static constexpr size_t smem = (size_t)teams * 8 * TPR * NV * 4 * sizeof(float);
+    static constexpr size_t smem = (size_t)teams * 8 * (TPR * NV * 4 + 4) * sizeof(float);
     static auto kernel(bool vec, bool general) {
         return vec ? (general ? norm_residual_bwd_kernel<TPR, NV, true, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, true, false, CLUSTER>)
                    : (general ? norm_residual_bwd_kernel<TPR, NV, false, true, CLUSTER> : norm_residual_bwd_kernel<TPR, NV, false, false, CLUSTER>);
     }
     // blocks (clusters of `csize`) that the device holds at once; 0 with the error set
     static int resident(int dev, bool vec, bool general, unsigned csize) {
-        static int known[EDDLB200_MAX_DEVICES][4][5] = {};
+        static int known[EDDLB200_MAX_DEVICES][4][kMaxCluster + 1] = {};
         int &n = known[dev][2 * vec + general][csize];
         if (n) return n;
         auto k = kernel(vec, general);
@@ -477,7 +514,7 @@ auto with_bwd(int cols, Go go) {
     if (cols <= 1024) return go(Bwd<128, 2, false>());
     if (cols <= 2048) return go(Bwd<256, 2, false>());
     if (cols <= 4096) return go(Bwd<512, 2, false>());
-    return go(Bwd<512, 2, true>());
+    return go(Bwd<256, 2, true>());
 }
 
 // An output may be an input's own memory (every value is read before it is written, by the thread that writes it), but not part of it.
@@ -558,7 +595,7 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
     }
     EB_CTX(dev);
     const bool cluster = cols > 4096, general = kind || db1 || db2;
-    const unsigned csize = cluster ? (unsigned)ceil_div(cols, 4096) : 1;
+    const unsigned csize = cluster ? (unsigned)ceil_div(cols, 2048) : 1;
     bool vec = cols % 4 == 0;
     for (int i = 0; i < 8; i++) vec = vec && aligned16(in[i]);
     vec = vec && aligned16(df) && aligned16(dr);
