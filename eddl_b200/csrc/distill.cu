@@ -23,14 +23,14 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxPiece = 43008;                 // logits of a row in one block: 168 KB of shared memory, with up to 44 KB of entries
+constexpr int kMaxPiece = 43008;                 // logits of a row in one block: 168 KB of shared memory, with up to 36 KB of entries
 constexpr int kMaxCols = kMaxPiece * kMaxCluster;
 
 struct Args {
     const float *x, *teacher, *teacher_lse, *weights;
     const int *ids, *labels;
     float *loss, *delta;
-    int rows, cols, k, piece, slots;             // piece: logits of one block, a multiple of 4; slots: of the table of ids seen, a power of two
+    int rows, cols, k, piece;                    // piece: logits of one block, a multiple of 4
     size_t ld;
     float temperature, alpha;
 };
@@ -84,8 +84,8 @@ struct Ahead {
     }
 };
 
-// One warp: the record of a row.  `table`: slots that hold -1, and do so again afterwards.
-__device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, const Record &r, int *table, int *slot_of) {
+// One warp: the record of a row.
+__device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, const Record &r) {
     const int lane = threadIdx.x & 31;
     __syncwarp();                                // the record may be an earlier row's that a lane of this warp still reads
     Ahead now = ahead;
@@ -104,7 +104,8 @@ __device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, cons
     float top = minus_inf(), anchor = minus_inf();
     bool label_seen = false;
     if (soft) {
-        // Of several entries with one id the first counts: the lowest lane of 32 at a time, and only if no earlier 32 had it.
+        // Of several entries with one id the first counts: the lowest lane of 32 at a time, and only if none of the earlier ones, which all lanes look
+        // through together, had it (k = 128: some 300 cycles; a table of the ids seen took ten times that).
         for (int j0 = 0; j0 < a.k; j0 += 32 * kAhead) {
             if (j0) now.entries(a, row, j0, lane);
             float value[kAhead];
@@ -117,20 +118,15 @@ __device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, cons
             for (int c = 0; c < kAhead; c++) {
                 const int j = j0 + c * 32 + lane;
                 if (j - lane >= a.k) break;
-                int id = now.id[c], slot = -1;
+                int id = now.id[c];
                 const unsigned same = __match_any_sync(0xffffffffu, id);
-                if (id >= 0 && (int)__ffs(same) - 1 != lane) id = -1;
-                if (id >= 0 && a.k > 32) {
-                    unsigned h = ((unsigned)id * 2654435761u) >> 12 & (a.slots - 1);
-                    for (;;) {                   // the table is at most half full: an empty slot is met
-                        const int old = atomicCAS(table + h, -1, id);
-                        if (old == -1) { slot = (int)h; break; }
-                        if (old == id) { id = -1; break; }
-                        h = (h + 1) & (a.slots - 1);
-                    }
-                }
+                bool seen = (int)__ffs(same) - 1 != lane;
+                const int4 *before = reinterpret_cast<const int4 *>(r.id);
+#pragma unroll 4
+                for (int q = 0; q < (j - lane) / 4; q++) { const int4 o = before[q]; seen |= o.x == id || o.y == id || o.z == id || o.w == id; }
+                if (seen) id = -1;
+                if (j < a.k) { r.id[j] = id; r.value[j] = value[c]; r.less[j] = now.t[c]; }
                 __syncwarp();
-                if (j < a.k) { r.id[j] = id; r.value[j] = value[c]; r.less[j] = now.t[c]; slot_of[j] = slot; }
                 if (id >= 0) { top = max_nan(top, now.t[c]); anchor = max_nan(anchor, value[c]); label_seen |= id == label; }
             }
         }
@@ -143,25 +139,21 @@ __device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, cons
     double sum = 0.0, terms = 0.0, per_sum = 1.0;
     float z = 0.f, z1 = 0.f;
     if (entries) {
+        const float c_t = kLog2e / a.temperature;
         for (int j = lane; j < a.k; j += 32) {
-            if (slot_of[j] >= 0) table[slot_of[j]] = -1;
             if (r.id[j] < 0) continue;
-            double log_p;
-            float p;
+            const float below = r.value[j] - anchor;
+            float log_p, p;
             if (tail) {                          // 1 - sum p may be small: in 64 bits up to the sum
-                log_p = (double)r.less[j] * inv_t - lse;
-                const double e = exp(log_p);
-                p = (float)e;
+                const double d = (double)r.less[j] * inv_t - lse, e = exp(d);
+                log_p = (float)d; p = (float)e;
                 sum += e;
-                const float below = r.value[j] - anchor;
-                z += exp2_fast(below * (kLog2e / a.temperature)); z1 += exp2_fast(below * kLog2e);
+                z += exp2_fast(below * c_t); z1 += exp2_fast(below * kLog2e);
             } else {
-                const float d = (r.less[j] - top) * (float)inv_t;
-                log_p = d;
-                p = expf(d);
+                log_p = (r.less[j] - top) * (float)inv_t; p = expf(log_p);
                 sum += p;
             }
-            if (p != 0.f) terms += (double)p * (log_p - ((double)r.value[j] - (double)anchor) * inv_t);
+            if (p != 0.f) terms += p * (log_p - below * (float)inv_t);
             r.less[j] = p;
         }
 #pragma unroll
@@ -171,7 +163,7 @@ __device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, cons
         const float scale = (float)(ws * per_sum);
         for (int j = lane; j < a.k; j += 32) r.less[j] *= scale;
     } else if (soft) {
-        for (int j = lane; j < a.k; j += 32) { if (slot_of[j] >= 0) table[slot_of[j]] = -1; r.id[j] = -1; }
+        for (int j = lane; j < a.k; j += 32) r.id[j] = -1;
     }
     label_seen = __any_sync(0xffffffffu, entries && label_seen);
     if (lane == 0) {
@@ -206,7 +198,7 @@ struct Run {
 // of a cluster.  16-byte accesses whatever the row's alignment: the piece is laid out in shared memory with the alignment it has in
 // global memory, -infinity around it, so the sums need no bounds.  A thread copies (cp.async), sums and writes the same pieces of the row, so
 // between those steps nobody waits.  ex2 of one product: 2^-22 relative, the argument's roundings as in any fp32 softmax.
-constexpr int blocks_per_sm(int team) { return team == 32 ? 5 : team == 128 ? 8 : 3; }
+constexpr int blocks_per_sm(int team) { return team == 32 ? 4 : team == 128 ? 6 : 3; }
 template <int TEAM, bool CLUSTER>
 __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TEAM)) distill_kernel(const Args a) {
     constexpr bool OWN = TEAM == 32;                       // every warp its own rows, entries and all
@@ -216,8 +208,7 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
     __shared__ float4 runs[OWN ? 1 : 2][CLUSTER ? kMaxCluster : 1][W];
     const int team = OWN ? threadIdx.x / 32 : 0, t = OWN ? threadIdx.x % 32 : threadIdx.x, lane = threadIdx.x & 31, warp = t >> 5;
     const int kk = (a.k + 3) & ~3;
-    float *x = smem + (size_t)team * (a.piece + 4 + (3 * RECORDS + 1) * kk + a.slots), *lists = x + a.piece + 4;
-    int *slot_of = reinterpret_cast<int *>(lists + 3 * RECORDS * kk), *table = slot_of + kk;
+    float *x = smem + (size_t)team * (a.piece + 4 + 3 * RECORDS * kk), *lists = x + a.piece + 4;
     auto record = [&](int i) {
         float *p = lists + 3 * kk * i;
         return Record{heads + team + i, p, p + kk, reinterpret_cast<int *>(p + 2 * kk)};
@@ -229,8 +220,6 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
     auto meeting = [&]() { if (CLUSTER) cg::this_cluster().sync(); else if (OWN) __syncwarp(); else __syncthreads(); };
     auto team_barrier = [&]() { if (OWN) __syncwarp(); else asm volatile("bar.sync 1, %0;" ::"n"(TEAM) : "memory"); };
     const int first = (int)(blockIdx.x / csize) * TEAMS + team, step = (int)(gridDim.x / csize) * TEAMS;
-    if (OWN || warp == W) for (int i = lane; i < a.slots; i += 32) table[i] = -1;
-    __syncwarp();
     EB_GRID_WAIT();
 
     // the row's maximum and sums from its warps' lines; with the entries' cells closed the maximum is theirs too
@@ -267,14 +256,14 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
         // ============================ the entries, one row ahead; the loss ============================
         Ahead ahead;
         ahead.ask(a, first);
-        if (first < a.rows) look_up(a, first, first + step, ahead, record(0), table, slot_of);
+        if (first < a.rows) look_up(a, first, first + step, ahead, record(0));
         meeting();
         int i = 0, flip = 0;
         for (int row = first; row < a.rows; row += step, flip ^= 1) {
             const Head &h = *record(i).head;
             // the record written here was last read two meetings ago
             i = i == 2 ? 0 : i + 1;
-            if (row + step < a.rows) look_up(a, row + step, row + 2 * step, ahead, record(i), table, slot_of);
+            if (row + step < a.rows) look_up(a, row + step, row + 2 * step, ahead, record(i));
             meeting();
             if (rank) continue;
             float loss = 0.f;
@@ -310,7 +299,7 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
         if (!OWN) meeting();
         for (int row = first; row < a.rows; row += step, flip ^= 1) {
             const Record r = record(i);
-            if (OWN) look_up(a, row, row + step, ahead, r, table, slot_of);
+            if (OWN) look_up(a, row, row + step, ahead, r);
             else i = i == 2 ? 0 : i + 1;
             float *dst = a.delta ? a.delta + (size_t)row * a.ld + c0 : nullptr;
             const bool live = r.head->live != 0;
@@ -489,10 +478,9 @@ extern "C" int eddlb200_distill(int dev, const float *logits, const int *ids, co
     if (ld == (size_t)cols) EB_WRITES(delta, bytes); else EB_MODIFIES(delta, bytes);
     EB_WRITES(loss, each);
     ProfScope prof(cx, PROF_ELEMENTWISE, (delta ? 8.0 : 4.0) * rows * cols);
-    Args a{logits, teacher, teacher_lse, weights, ids, labels, loss, delta, rows, cols, k, 0, 64, ld, temperature, alpha};
-    while (a.slots < 2 * k) a.slots *= 2;
+    Args a{logits, teacher, teacher_lse, weights, ids, labels, loss, delta, rows, cols, k, 0, ld, temperature, alpha};
     const size_t kk = (k + 3) & ~3;
-    auto smem = [&](unsigned c, int records) { a.piece = (int)((ceil_div(cols, c) + 3) & ~(size_t)3); return ((size_t)a.piece + 4 + (3 * records + 1) * kk + a.slots) * sizeof(float); };
+    auto smem = [&](unsigned c, int records) { a.piece = (int)((ceil_div(cols, c) + 3) & ~(size_t)3); return ((size_t)a.piece + 4 + 3 * records * kk) * sizeof(float); };
     if (cols <= 256 || (cols <= 1024 && rows >= EDDLB200_NUM_SMS * 16)) { const size_t b = 8 * smem(1, 1); return launch_distill<32, false>(cx, dev, st, a, 1, b); }
     if (cols <= 4096) { const size_t b = smem(1, 3); return launch_distill<128, false>(cx, dev, st, a, 1, b); }
     if (cols <= 16384) { const size_t b = smem(1, 3); return launch_distill<256, false>(cx, dev, st, a, 1, b); }
