@@ -9,7 +9,7 @@
 //
 // Bound by memory: 8 bytes a logit.  A row lies in shared memory between its one read and its one write -- of one block, or in
 // pieces in the blocks of a cluster.  What has to do with the entries (a few dozen a row: look-ups, repeated ids, 64-bit
-// exponentials) is a chain of latencies as long as the streaming of the row, so it has a warp of its own that works one row ahead; the
+// exponentials) is a chain of latencies as long as the streaming of the row, so it has a warp of its own that works ahead; the
 // other warps keep a running maximum and sum a thread and meet once a row.  Mass outside the entries is summed from the
 // values outside, not as 1 minus something: with `teacher_lse` the entries' cells are set to -infinity before the sum.
 #include <type_traits>
@@ -59,6 +59,7 @@ struct Head {
     double base, per_z, per_rest, hard;
     float inside, rest, x_label, anchor;         // anchor: the largest of the entries' logits
     float z, z1;                                 // the entries' sums relative to it, where their cells are closed
+    float row_m, row_out, row_z, row_z1;         // what the other warps found of the row: m, z_out, z, z_1; m = -infinity: nothing that counts
     int label, label_is_entry, live;
 };
 struct Record {
@@ -204,13 +205,15 @@ struct Run {
 // of a cluster.  16-byte accesses whatever the row's alignment: the piece is laid out in shared memory with the alignment it has in
 // global memory, -infinity around it, so the sums need no bounds.  A thread copies (cp.async), sums and writes the same pieces of the row, so
 // between those steps nobody waits.  ex2 of one product: 2^-22 relative, the argument's roundings as in any fp32 softmax.
-constexpr int blocks_per_sm(int team) { return team == 32 ? 4 : team == 128 ? 6 : 3; }
+constexpr int blocks_per_sm(int team) { return team == 32 ? 4 : team == 128 ? 4 : 3; }
+constexpr int entry_warps(bool cluster) { return cluster ? 1 : 2; }
+constexpr int block_of(int team, bool cluster) { return team == 32 ? 256 : team + 32 * entry_warps(cluster); }
 template <int TEAM, bool CLUSTER>
-__global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TEAM)) distill_kernel(const Args a) {
+__global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) distill_kernel(const Args a) {
     constexpr bool OWN = TEAM == 32;                       // every warp its own rows, entries and all
-    constexpr int TEAMS = OWN ? 8 : 1, W = TEAM / 32, RECORDS = OWN ? 1 : 3;
+    constexpr int TEAMS = OWN ? 8 : 1, W = TEAM / 32, RECORDS = OWN ? 1 : CLUSTER ? 3 : 4;
     extern __shared__ __align__(16) float smem[];
-    __shared__ Head heads[OWN ? 8 : 3];
+    __shared__ Head heads[OWN ? 8 : RECORDS];
     __shared__ float4 runs[OWN ? 1 : 2][CLUSTER ? kMaxCluster : 1][W];
     const int team = OWN ? threadIdx.x / 32 : 0, t = OWN ? threadIdx.x % 32 : threadIdx.x, lane = threadIdx.x & 31, warp = t >> 5;
     const int kk = (a.k + 3) & ~3;
@@ -223,7 +226,12 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
     const int c0 = rank * a.piece, n = max(0, min(a.piece, a.cols - c0));
     const bool tail = a.teacher_lse != nullptr && a.alpha != 1.f, one_exp = a.temperature == 1.f, any_entries = a.alpha != 1.f;
     const float c_t = kLog2e / a.temperature;
-    auto meeting = [&]() { if (CLUSTER) cg::this_cluster().sync(); else if (OWN) __syncwarp(); else __syncthreads(); };
+    // Clusters: all threads of all blocks meet once a row, the one entry warp with the next row's record.  Single blocks: the records are passed on by
+    // barriers of their own (2 + i: record i is there, 6 + i: it has been used), between the team and one of two entry warps that
+    // take the rows in turn; beside busy warps a look-up takes 8 to 13 k cycles, several times its row where rows are short.
+    auto meeting = [&]() { if (CLUSTER) cg::this_cluster().sync(); };
+    auto wait_for = [&](int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(TEAM + 32) : "memory"); };
+    auto tell = [&](int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(TEAM + 32) : "memory"); };
     auto team_barrier = [&]() { if (OWN) __syncwarp(); else asm volatile("bar.sync 1, %0;" ::"n"(TEAM) : "memory"); };
     const int first = (int)(blockIdx.x / csize) * TEAMS + team, step = (int)(gridDim.x / csize) * TEAMS;
     EB_GRID_WAIT();
@@ -249,36 +257,54 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
         run.meet(top, c_t); own.meet(top, c_t);
         return own;
     };
-    auto loss_of = [&](const Head &h, const Run &run, const Run &own) {
-        const float z = run.z + own.z, z1 = one_exp && any_entries ? z : run.z1 + own.z1;
+    auto loss_of = [&](const Head &h, float m, float z_out, float z, float z1) {
         double l = h.base;
-        if (any_entries) l += h.per_z * (((double)run.m - (double)h.anchor) / (double)a.temperature + (double)logf(z));
-        if (h.per_rest > 0.0) l -= h.per_rest * ((double)logf(run.z) - (double)logf(z));
-        if (h.label >= 0) l += h.hard * ((double)run.m - (double)h.x_label + (double)logf(z1));
+        if (any_entries) l += h.per_z * (((double)m - (double)h.anchor) / (double)a.temperature + (double)logf(z));
+        if (h.per_rest > 0.0) l -= h.per_rest * ((double)logf(z_out) - (double)logf(z));
+        if (h.label >= 0) l += h.hard * ((double)m - (double)h.x_label + (double)logf(z1));
         return (float)l;
     };
 
-    if (!OWN && warp == W) {
-        // ============================ the entries, one row ahead; the loss ============================
-        Ahead ahead;
-        ahead.ask(a, first);
-        if (first < a.rows) look_up(a, first, first + step, ahead, record(0));
-        meeting();
-        int i = 0, flip = 0;
-        for (int row = first; row < a.rows; row += step, flip ^= 1) {
-            const Head &h = *record(i).head;
-            // the record written here was last read two meetings ago
-            i = i == 2 ? 0 : i + 1;
-            if (row + step < a.rows) look_up(a, row + step, row + 2 * step, ahead, record(i));
+    if (!OWN && warp >= W) {
+        // ============================ the entries, ahead of their rows; the loss ============================
+        if (CLUSTER) {
+            Ahead ahead;
+            ahead.ask(a, first);
+            if (first < a.rows) look_up(a, first, first + step, ahead, record(0));
             meeting();
-            if (rank) continue;
-            float loss = 0.f;
-            if (h.live) {
-                Run run = combine(flip);
-                const Run own = add_entries(run, h);
-                if (run.m != minus_inf()) loss = loss_of(h, run, own);
+            int i = 0, flip = 0;
+            for (int row = first; row < a.rows; row += step, flip ^= 1) {
+                const Head &h = *record(i).head;
+                // the record written here was last read two meetings ago
+                i = i == 2 ? 0 : i + 1;
+                if (row + step < a.rows) look_up(a, row + step, row + 2 * step, ahead, record(i));
+                meeting();
+                if (rank) continue;
+                float loss = 0.f;
+                if (h.live) {
+                    Run run = combine(flip);
+                    const Run own = add_entries(run, h);
+                    const float z = run.z + own.z;
+                    if (run.m != minus_inf()) loss = loss_of(h, run.m, run.z, z, one_exp && any_entries ? z : run.z1 + own.z1);
+                }
+                if (lane == 0) a.loss[row] = loss;
             }
-            if (lane == 0) a.loss[row] = loss;
+        } else {
+            auto finish = [&](int n) {                       // row n of the block is done: its loss, and its record may be written again
+                wait_for(6 + (n & 3));
+                const Head &h = *record(n & 3).head;
+                const float loss = h.row_m == minus_inf() ? 0.f : loss_of(h, h.row_m, h.row_out, h.row_z, h.row_z1);
+                if (lane == 0) a.loss[first + n * step] = loss;
+            };
+            Ahead ahead;
+            int n = warp - W;
+            ahead.ask(a, first + n * step);
+            for (; first + n * step < a.rows; n += 2) {
+                if (n >= 4) finish(n - 4);
+                look_up(a, first + n * step, first + (n + 2) * step, ahead, record(n & 3));
+                tell(2 + (n & 3));
+            }
+            for (int m = n >= 4 ? n - 4 : n - 2; m < n; m += 2) if (m >= 0) finish(m);
         }
     } else {
         // piece v of the row, 16 bytes, on its way into its place; -infinity where there is no logit
@@ -302,11 +328,22 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
         Ahead ahead;
         if (OWN) ahead.ask(a, first);
         fetch_row(first);
-        if (!OWN) meeting();
+        meeting();
         for (int row = first; row < a.rows; row += step, flip ^= 1) {
             const Record r = record(i);
+            const int turn = i;
             if (OWN) look_up(a, row, row + step, ahead, r);
-            else i = i == 2 ? 0 : i + 1;
+            else i = i == RECORDS - 1 ? 0 : i + 1;
+            if (!OWN && !CLUSTER) wait_for(2 + turn);
+            auto done = [&](float m, float z_out, float z, float z1) {
+                if (OWN) {
+                    if (t == 0) a.loss[row] = m == minus_inf() ? 0.f : loss_of(*r.head, m, z_out, z, z1);
+                    __syncwarp();
+                } else if (!CLUSTER) {
+                    if (t == 0) { r.head->row_m = m; r.head->row_out = z_out; r.head->row_z = z; r.head->row_z1 = z1; }
+                    tell(6 + turn);
+                }
+            };
             float *dst = a.delta ? a.delta + (size_t)row * a.ld + c0 : nullptr;
             const bool live = r.head->live != 0;
             const int off = misfit(source(row)), end = off + n, nv = (end + 3) >> 2, label = live ? r.head->label : -1;
@@ -354,7 +391,7 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
                 }
             }
             if (!OWN) {
-                meeting();
+                if (CLUSTER) meeting(); else team_barrier();
                 if (live) run = combine(flip);
             }
             Run own{};
@@ -362,12 +399,11 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
             if (!live || run.m == minus_inf()) {           // no weight, or a mask leaves nothing of the row
                 fetch_row(row + step);
                 if (dst) for (int q = t; q < n; q += TEAM) dst[q] = 0.f;
-                if (OWN && t == 0) a.loss[row] = 0.f;
+                done(minus_inf(), 0.f, 0.f, 0.f);
                 continue;
             }
-            if (OWN && t == 0) a.loss[row] = loss_of(*r.head, run, own);
-            if (!dst) { fetch_row(row + step); if (OWN) __syncwarp(); continue; }
             const float m = run.m, z_out = run.z, z = z_out + own.z, z1 = one_exp && any_entries ? z : run.z1 + own.z1;
+            if (!dst) { fetch_row(row + step); done(m, z_out, z, z1); continue; }
             const float f_in = any_entries ? r.head->inside / z : 0.f, f_1 = ce ? (float)r.head->hard / z1 : 0.f;
             const float f_out = tail ? (z_out > 0.f ? f_in - r.head->rest / z_out : 0.f) : f_in;
             const bool straight = misfit(dst) == off;
@@ -419,7 +455,7 @@ __global__ void __launch_bounds__(TEAM == 32 ? 256 : TEAM + 32, blocks_per_sm(TE
                 const float d = r.head->x_label - m;
                 dst[label - c0] = f_1 * exp2_fast(d * kLog2e) + f_out * exp2_fast(d * c_t) - hard;
             }
-            if (OWN) __syncwarp();
+            done(m, z_out, z, z1);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     }
@@ -435,7 +471,7 @@ int launch_distill(DevCtx *cx, int dev, cudaStream_t st, const Args &a, unsigned
         if (e != cudaSuccess) return cuda_status(e, "distill(attributes)");
         configured[dev] = true;
     }
-    constexpr int block = TEAM == 32 ? 256 : TEAM + 32, teams = TEAM == 32 ? 8 : 1;
+    constexpr int block = block_of(TEAM, CLUSTER), teams = TEAM == 32 ? 8 : 1;
     size_t per_sm = (size_t)227 * 1024 / (smem + 4 * 1024);
     if (per_sm > (size_t)blocks_per_sm(TEAM)) per_sm = blocks_per_sm(TEAM);
     if (per_sm < 1) per_sm = 1;
@@ -477,7 +513,7 @@ extern "C" int eddlb200_distill(int dev, const float *logits, const int *ids, co
     EB_REQUIRE(temperature >= 1.17549435e-38f && temperature < INFINITY, what);
     EB_REQUIRE(alpha >= 0.f && alpha <= 1.f, what);
     if (cols > kMaxCols) return set_error(EDDLB200_ELIMIT, "%s: %d classes, at most %d", what, cols, kMaxCols);
-    if (rows > 0x7fff0000) return set_error(EDDLB200_ELIMIT, "%s: %d rows", what, rows);
+    if (rows > 0x7ff00000) return set_error(EDDLB200_ELIMIT, "%s: %d rows", what, rows);
     if (k > kMaxTop) return set_error(EDDLB200_ELIMIT, "%s: %d entries a row, at most %d", what, k, kMaxTop);
     EB_REQUIRE(!rows || (logits && ids && teacher && loss), what);
     EB_REQUIRE(!rows || labels || alpha == 0.f, what);
@@ -498,9 +534,11 @@ extern "C" int eddlb200_distill(int dev, const float *logits, const int *ids, co
     Args a{logits, teacher, teacher_lse, weights, ids, labels, loss, delta, rows, cols, k, 0, ld, temperature, alpha};
     const size_t kk = (k + 3) & ~3;
     auto smem = [&](unsigned c, int records) { a.piece = (int)((ceil_div(cols, c) + 3) & ~(size_t)3); return ((size_t)a.piece + 4 + 3 * records * kk) * sizeof(float); };
-    if (cols <= 256 || (cols <= 1024 && rows >= EDDLB200_NUM_SMS * 16)) { const size_t b = 8 * smem(1, 1); return launch_distill<32, false>(cx, dev, st, a, 1, b); }
-    if (cols <= 4096) { const size_t b = smem(1, 3); return launch_distill<128, false>(cx, dev, st, a, 1, b); }
-    if (cols <= 16384) { const size_t b = smem(1, 3); return launch_distill<256, false>(cx, dev, st, a, 1, b); }
+    // A warp a row, entries and all, as long as two blocks of eight rows fit an SM and there are rows for every SM: nothing waits for anything but its own
+    // latencies (40000 x 1300, 32 entries: 119 us, with a block a row 233; 16384 x 4000, where one block fits: 180 and 147).
+    if (cols <= 256 || (8 * smem(1, 1) <= 112 * 1024 && rows >= EDDLB200_NUM_SMS * 8)) { const size_t b = 8 * smem(1, 1); return launch_distill<32, false>(cx, dev, st, a, 1, b); }
+    if (cols <= 8192) { const size_t b = smem(1, 4); return launch_distill<128, false>(cx, dev, st, a, 1, b); }
+    if (cols <= 16384) { const size_t b = smem(1, 4); return launch_distill<256, false>(cx, dev, st, a, 1, b); }
     const unsigned csize = cols <= 32768 ? 2 : cols <= 65536 ? 4 : 8;
     const size_t b = smem(csize, 3);
     return launch_distill<256, true>(cx, dev, st, a, csize, b);
