@@ -198,6 +198,8 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const CUtensorMap
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst_smem), "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// the copy engine's look at a map, ahead of its first copy
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory"); }
 __device__ __forceinline__ void umma_fp8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
@@ -233,6 +235,7 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, ProdShape<BN>::PER_SM)
         for (int s = 0; s < S::BUFS; s++) { mbar_init(bar_acc_full + 8 * s, 1); mbar_init(bar_acc_empty + 8 * s, S::EPI); }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&P.map_p); prefetch_map(&P.map_q);
     }
     if (warp == 1) tmem_alloc(smem_u32(&tmem_slot), S::TMEM);
     EB_GRID_WAIT();
@@ -436,6 +439,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
         for (int s = 0; s < 2; s++) { mbar_init(bar_acc_full + 8 * s, 1); mbar_init(bar_acc_empty + 8 * s, 32); }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&P.map_p); prefetch_map(&P.map_q);
     }
     if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_slot), 512);
     EB_GRID_WAIT();
@@ -637,18 +641,48 @@ bool encode_bytes_map(CUtensorMap *map, const void *base, size_t ld, int rows, i
 }
 
 template <int BN>
-int launch_product(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P, unsigned tiles) {
-    static bool configured[EDDLB200_MAX_DEVICES] = {};
+int launch_product(DevCtx *cx, cudaStream_t st, const ProdParams &P, unsigned tiles) {
     using S = ProdShape<BN>;
-    if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(fp8_product_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-        if (e != cudaSuccess) return cuda_status(e, "fp8_mult2d(attributes)");
-        configured[dev] = true;
-    }
     if (P.splits > 1) eb::launch_cluster(fp8_product_kernel<BN>, (unsigned)P.splits, tiles * P.splits, S::THREADS, S::SMEM, st, P);
     else eb::launch(fp8_product_kernel<BN>, tiles, S::THREADS, S::SMEM, st, P);
     EB_LAUNCH_CHECK("fp8_mult2d");
-    g_fp8_used[dev] = true;
+    return 0;
+}
+
+// What the device holds at once of each tile's kernel: clusters of 1 .. 8 blocks.  A cluster lies within one group of SMs, so their number is not that of
+// the blocks divided by the size (1 x 6000 x 6000: 47 clusters of six are two rounds, 15.6 us, 47 of five one, 11.2).  Looked up with the first product on a
+// device, along with the kernels' attributes.  The query counts one block an SM of a kernel that uses tensor memory; two of the small tiles' are there
+// (10.3 warps of blocks of six active on an SM in a profile of 1 x 8192 x 8192), so its numbers of clusters are doubled.
+struct Residents { bool known = false; int of[5][9]; };
+Residents g_residents[EDDLB200_MAX_DEVICES];
+template <int BN>
+cudaError_t look_up_residents(int (&of)[9]) {
+    using S = ProdShape<BN>;
+    cudaError_t e = cudaFuncSetAttribute(fp8_product_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&of[1], fp8_product_kernel<BN>, S::THREADS, S::SMEM);
+    const int twice = e == cudaSuccess && of[1] == 1 ? S::PER_SM : 1;
+    of[1] *= twice * EDDLB200_NUM_SMS;
+    for (int size = 2; size <= 8 && e == cudaSuccess; size++) {
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension; at[0].val.clusterDim.x = size; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t c = {};
+        c.gridDim = dim3(EDDLB200_NUM_SMS * S::PER_SM / size * size); c.blockDim = dim3(S::THREADS); c.dynamicSmemBytes = S::SMEM; c.attrs = at; c.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&of[size], fp8_product_kernel<BN>, &c);
+        of[size] *= twice;
+    }
+    return e;
+}
+int product_residents(int dev, const Residents *&out) {
+    Residents &r = g_residents[dev];
+    out = &r;
+    if (r.known) return 0;
+    cudaError_t e = look_up_residents<16>(r.of[0]);
+    if (e == cudaSuccess) e = look_up_residents<32>(r.of[1]);
+    if (e == cudaSuccess) e = look_up_residents<64>(r.of[2]);
+    if (e == cudaSuccess) e = look_up_residents<128>(r.of[3]);
+    if (e == cudaSuccess) e = look_up_residents<256>(r.of[4]);
+    if (e != cudaSuccess) return cuda_status(e, "fp8_mult2d(occupancy)");
+    r.known = true;
     return 0;
 }
 
@@ -657,17 +691,19 @@ int launch_product(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P, un
 // wide tiles, the epilogue's; alone on its SM a block waits at least for its own chain.  A tile costs its start and its stores and, when split,
 // the exchange between the blocks of a cluster.  256 x 4096 x 4096: 128 rows in two splits 15.8 us, pairs 22.0; 2048 cubed: pairs 16.0, 256 rows 24.8.
 struct Plan { int bn = 0, splits = 1; size_t tiles = 0; };           // bn 0: the kernel on pairs of CTAs
-Plan pick_plan(int m, int n, int kblocks) {
+Plan pick_plan(const Residents &held, int m, int n, int kblocks) {
     Plan best;
     best.tiles = ceil_div(m, 256) * ceil_div(n, 256);
     double least = (double)ceil_div(best.tiles, (size_t)EDDLB200_NUM_SMS / 2) * (1050.0 * kblocks + 8000.0);
     for (int bn = 16; bn <= 256; bn *= 2) {
         if (bn > 16 && bn / 2 >= m) break;                           // half of the tile would be empty
-        const size_t tiles = ceil_div(n, 128) * ceil_div(m, bn), slots = (size_t)EDDLB200_NUM_SMS * (bn <= 64 ? 2 : 1);
+        const int which = bn == 16 ? 0 : bn == 32 ? 1 : bn == 64 ? 2 : bn == 128 ? 3 : 4;
+        const size_t tiles = ceil_div(n, 128) * ceil_div(m, bn);
         const double block = bn == 16 ? 410.0 : bn == 32 ? 450.0 : bn == 64 ? 580.0 : bn == 128 ? 950.0 : 1800.0;
         const double alone = bn == 16 ? 600.0 : bn == 32 ? 720.0 : bn == 64 ? 950.0 : block;
         for (int splits = 1; splits <= 8 && splits <= kblocks; splits++) {
-            const size_t jobs = tiles * splits, rounds = ceil_div(jobs, slots), on_one = ceil_div(jobs, (size_t)EDDLB200_NUM_SMS);
+            if (held.of[which][splits] < 1) continue;
+            const size_t jobs = tiles * splits, rounds = ceil_div(tiles, (size_t)held.of[which][splits]), on_one = ceil_div(jobs, (size_t)EDDLB200_NUM_SMS);
             const double each = (double)ceil_div(kblocks, splits);
             const double work = on_one > 1 ? on_one * each * block : each * alone;
             const double t = work + rounds * (4000.0 + 25.0 * bn + (splits > 1 ? 700.0 * splits + 8.0 * bn : 0.0));
@@ -774,7 +810,10 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
         return encode_bytes_map(&P.map_p, p.q, p.ld, p.rows, k, p_box) && encode_bytes_map(&P.map_q, q.q, q.ld, q.rows, k, q_box);
     };
     const char *const refused = "%s: the driver refuses a tensor map of the operands";
-    const Plan plan = pick_plan(m, n, P.kblocks);
+    const Residents *held;
+    if (int e = product_residents(dev, held)) return e;
+    const Plan plan = pick_plan(*held, m, n, P.kblocks);
+    g_fp8_used[dev] = true;
     if (plan.tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
     if (!plan.bn) {
         const bool rows = block_b == kBlk, vec = !rows && block_a != kBlk;
@@ -788,11 +827,11 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     P.tiles_p = (int)ceil_div(n, 128); P.splits = plan.splits;
     P.idesc = fp8_idesc(format_b, format_a, 128, bn);
     switch (bn) {
-        case 16: return launch_product<16>(cx, dev, st, P, (unsigned)plan.tiles);
-        case 32: return launch_product<32>(cx, dev, st, P, (unsigned)plan.tiles);
-        case 64: return launch_product<64>(cx, dev, st, P, (unsigned)plan.tiles);
-        case 128: return launch_product<128>(cx, dev, st, P, (unsigned)plan.tiles);
-        default: return launch_product<256>(cx, dev, st, P, (unsigned)plan.tiles);
+        case 16: return launch_product<16>(cx, st, P, (unsigned)plan.tiles);
+        case 32: return launch_product<32>(cx, st, P, (unsigned)plan.tiles);
+        case 64: return launch_product<64>(cx, st, P, (unsigned)plan.tiles);
+        case 128: return launch_product<128>(cx, st, P, (unsigned)plan.tiles);
+        default: return launch_product<256>(cx, st, P, (unsigned)plan.tiles);
     }
 }
 
