@@ -212,6 +212,7 @@ inline bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes
 }
 
 __host__ __device__ inline bool aligned16(const void *p) { return (((uintptr_t)p) & 15u) == 0; }
+__host__ __device__ inline bool aligned4(const void *p) { return (((uintptr_t)p) & 3u) == 0; }
 
 #ifdef __CUDACC__
 // Every kernel of the library is launched with programmatic stream serialisation: its blocks may be set up while the kernel

@@ -522,6 +522,8 @@ extern "C" int eddlb200_distill(int dev, const float *logits, const int *ids, co
     const size_t in_bytes[] = {entries, entries, each, each, each};
     EB_REQUIRE(delta == logits || !overlap(delta, bytes, logits, bytes), what);
     EB_REQUIRE(!overlap(loss, each, logits, bytes) && !overlap(loss, each, delta, bytes), what);
+    EB_REQUIRE(aligned4(logits) && aligned4(delta) && aligned4(loss), what);
+    for (int i = 0; i < 5; i++) EB_REQUIRE(aligned4(in[i]), what);
     for (int i = 0; i < 5; i++) EB_REQUIRE(!overlap(delta, bytes, in[i], in_bytes[i]) && !overlap(loss, each, in[i], in_bytes[i]), what);
     EB_CTX(dev);
     if (!rows) return 0;

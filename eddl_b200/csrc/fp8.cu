@@ -747,6 +747,7 @@ int eddlb200_fp8_quantize(int dev, const float *a, int rows, int cols, int forma
     EB_REQUIRE(!rows || !cols || a, what);
     const size_t tiles = ceil_div(rows, kBlk) * ceil_div(cols, kBlk);
     if (rows > kMaxSide || cols > kMaxSide || tiles > 0x7fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, rows, cols);
+    EB_REQUIRE(aligned4(a) && aligned4(scale) && aligned4(scale_t), what);
     const size_t in = (size_t)rows * cols * sizeof(float);
     const void *out[] = {q, scale, qt, scale_t};
     const size_t bytes[] = {matrix_bytes(rows, cols, ldq), scale_bytes(rows, cols, block_rows), matrix_bytes(cols, rows, ldqt), scale_bytes(cols, rows, block_rows)};
@@ -781,6 +782,7 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     EB_REQUIRE(lda < ((size_t)1 << 40) && ldb < ((size_t)1 << 40), what);
     EB_REQUIRE(!m || !n || c, what);
     EB_REQUIRE(!m || !n || !k || (qa && qb && scale_a && scale_b && aligned16(qa) && aligned16(qb)), what);
+    EB_REQUIRE(aligned4(c) && aligned4(scale_a) && aligned4(scale_b), what);
     if (m > kMaxSide || n > kMaxSide || k > kMaxSide) return set_error(EDDLB200_ELIMIT, "%s: %d x %d x %d", what, m, n, k);
     const size_t out = (size_t)m * n * sizeof(float);
     const void *in[] = {qa, qb, scale_a, scale_b};
@@ -788,18 +790,8 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     for (int i = 0; i < 4; i++) EB_REQUIRE(!overlap(c, out, in[i], bytes[i]), what);
     EB_CTX(dev);
     if (!m || !n) return 0;
-    for (int i = 0; i < 4; i++) EB_READS(in[i], bytes[i]);
-    if (!inc_c) EB_WRITES(c, out);
-    else {
-        EB_SETTLE(c, out);
-        int status = 0;
-        if (lz_take(cx, st, c, out, &status)) inc_c = 0;               // zeros owed to all of C: nothing to add to
-        if (status) return status;
-    }
-    ProfScope prof(cx, PROF_GEMM, 2.0 * m * n * k);
-    if (!k) return inc_c ? 0 : launch_zero_fill(cx, st, c, (size_t)m * n);
     ProdParams P;
-    P.c = c; P.kblocks = (int)ceil_div(k, kBlk); P.inc = inc_c != 0;
+    P.c = c; P.kblocks = (int)ceil_div(k, kBlk);
     struct Side { const void *q; size_t ld; const float *scale; int rows, block, format; };
     const Side sa{qa, lda, scale_a, m, block_a, format_a}, sb{qb, ldb, scale_b, n, block_b, format_b};
     auto sides = [&](const Side &p, const Side &q, int p_box, int q_box) {
@@ -809,24 +801,36 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
         P.p_scales = (int)ceil_div(p.rows, p.block); P.q_scales = (int)ceil_div(q.rows, q.block);
         return encode_bytes_map(&P.map_p, p.q, p.ld, p.rows, k, p_box) && encode_bytes_map(&P.map_q, q.q, q.ld, q.rows, k, q_box);
     };
-    const char *const refused = "%s: the driver refuses a tensor map of the operands";
-    const Residents *held;
-    if (int e = product_residents(dev, held)) return e;
-    const Plan plan = pick_plan(*held, m, n, P.kblocks);
-    g_fp8_used[dev] = true;
-    if (plan.tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
-    if (!plan.bn) {
-        const bool rows = block_b == kBlk, vec = !rows && block_a != kBlk;
-        if (!(rows ? sides(sa, sb, 128, 128) : sides(sb, sa, 128, 128))) return set_error(EDDLB200_EINVAL, refused, what);
-        P.tiles_p = (int)ceil_div(P.p_rows, 256); P.splits = (int)ceil_div(P.q_rows, 256);
-        P.idesc = rows ? fp8_idesc(format_a, format_b, 256, 256) : fp8_idesc(format_b, format_a, 256, 256);
-        return rows ? launch_large<false, true>(cx, dev, st, P) : vec ? launch_large<true, false>(cx, dev, st, P) : launch_large<false, false>(cx, dev, st, P);
+    Plan plan;
+    if (k) {
+        const Residents *held;
+        if (int e = product_residents(dev, held)) return e;
+        plan = pick_plan(*held, m, n, P.kblocks);
+        if (plan.tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
+        // C's rows are P's where only B's scales are shared by 128 rows: the side whose scales cost less is Q (see the kernel on pairs)
+        const bool rows = !plan.bn && block_b == kBlk;
+        if (!(plan.bn ? sides(sb, sa, 128, plan.bn) : rows ? sides(sa, sb, 128, 128) : sides(sb, sa, 128, 128)))
+            return set_error(EDDLB200_EINVAL, "%s: the driver refuses a tensor map of the operands", what);
+        P.tiles_p = (int)ceil_div(P.p_rows, plan.bn ? 128 : 256);
+        P.splits = plan.bn ? plan.splits : (int)ceil_div(P.q_rows, 256);
+        const int m_side = plan.bn ? 128 : 256, n_side = plan.bn ? plan.bn : 256;
+        P.idesc = rows ? fp8_idesc(format_a, format_b, m_side, n_side) : fp8_idesc(format_b, format_a, m_side, n_side);
     }
-    const int bn = plan.bn;
-    if (!sides(sb, sa, 128, bn)) return set_error(EDDLB200_EINVAL, refused, what);
-    P.tiles_p = (int)ceil_div(n, 128); P.splits = plan.splits;
-    P.idesc = fp8_idesc(format_b, format_a, 128, bn);
-    switch (bn) {
+    for (int i = 0; i < 4; i++) EB_READS(in[i], bytes[i]);
+    if (!inc_c) EB_WRITES(c, out);
+    else {
+        EB_SETTLE(c, out);
+        int status = 0;
+        if (lz_take(cx, st, c, out, &status)) inc_c = 0;               // zeros owed to all of C: nothing to add to
+        if (status) return status;
+    }
+    P.inc = inc_c != 0;
+    ProfScope prof(cx, PROF_GEMM, 2.0 * m * n * k);
+    if (!k) return inc_c ? 0 : launch_zero_fill(cx, st, c, (size_t)m * n);
+    g_fp8_used[dev] = true;
+    if (!plan.bn)
+        return block_b == kBlk ? launch_large<false, true>(cx, dev, st, P) : block_a == kBlk ? launch_large<false, false>(cx, dev, st, P) : launch_large<true, false>(cx, dev, st, P);
+    switch (plan.bn) {
         case 16: return launch_product<16>(cx, st, P, (unsigned)plan.tiles);
         case 32: return launch_product<32>(cx, st, P, (unsigned)plan.tiles);
         case 64: return launch_product<64>(cx, st, P, (unsigned)plan.tiles);

@@ -544,7 +544,9 @@ int eddlb200_norm_residual_fwd(int dev, int kind, int post, int groups, int rows
     EB_REQUIRE(!total || r, kFwd);
     const void *in[] = {f, r, gate, g1, b1, g2, b2};
     const size_t in_bytes[] = {bytes, bytes, gates, vector, vector, vector, vector};
+    EB_REQUIRE(aligned4(r_out) && aligned4(h), kFwd);
     for (int i = 0; i < 7; i++) {
+        EB_REQUIRE(aligned4(in[i]), kFwd);
         EB_REQUIRE(i < 2 ? !clash(r_out, bytes, in[i], in_bytes[i]) : !overlap(r_out, bytes, in[i], in_bytes[i]), kFwd);
         EB_REQUIRE(i < 2 ? !clash(h, bytes, in[i], in_bytes[i]) : !overlap(h, bytes, in[i], in_bytes[i]), kFwd);
         EB_REQUIRE(!overlap(stats, total * 16, in[i], in_bytes[i]), kFwd);
@@ -588,7 +590,9 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
     const size_t in_bytes[] = {bytes, bytes, bytes, bytes, gates, vector, vector, vector, total * 16};
     float *out[] = {df, dr, dgate, dg1, db1, dg2, db2};
     const size_t out_bytes[] = {bytes, bytes, gates, vector, vector, vector, vector};
+    for (int i = 0; i < 9; i++) EB_REQUIRE(aligned4(in[i]), kBwd);
     for (int o = 0; o < 7; o++) {
+        EB_REQUIRE(aligned4(out[o]), kBwd);
         for (int i = 0; i < 9; i++) EB_REQUIRE(o < 2 && i < 4 ? !clash(out[o], out_bytes[o], in[i], in_bytes[i]) : !overlap(out[o], out_bytes[o], in[i], in_bytes[i]), kBwd);
         for (int q = 0; q < o; q++) EB_REQUIRE(!overlap(out[o], out_bytes[o], out[q], out_bytes[q]), kBwd);
         EB_REQUIRE(!(o < 2 && inc_d && out[o]) || (out[o] != dh && out[o] != dr_out && out[o] != f && out[o] != r_out), kBwd);

@@ -107,7 +107,7 @@ def check(lib, wide, cols, ids, teacher, lse, labels, weights, T, alpha):
 
 
 SHAPES = [(1, 1, 0, 1), (3, 2, 1, 1), (5, 10, 0, 3), (40, 10, 2, 4), (9, 255, 0, 12), (8, 256, 4, 256), (7, 257, 0, 5), (64, 1000, 0, 10), (3, 1001, 3, 17), (2, 2048, 0, 130), (3, 2049, 0, 64),
-          (2, 16384, 0, 600), (2, 16387, 1, 33), (3, 32768, 0, 64), (2, 50001, 0, 1024), (1, 65537, 3, 100), (3, 131071, 1, 128), (1, 344064, 0, 16), (3000, 40, 0, 5), (700, 300, 0, 8)]
+          (2, 16384, 0, 600), (2, 16387, 1, 33), (3, 32768, 0, 64), (2, 50001, 0, 1024), (1, 65537, 3, 100), (3, 131071, 1, 128), (1, 344064, 0, 16), (3000, 40, 0, 5), (700, 300, 0, 8), (1300, 1301, 1, 9), (1250, 3000, 2, 40), (3000, 4501, 0, 7), (700, 20000, 2, 6)]
 
 
 @pytest.mark.parametrize("rows,cols,pad,k", SHAPES)

@@ -10,7 +10,7 @@ P = [0x10000000 * (i + 1) for i in range(24)]          # addresses far apart tha
 
 
 def call(name, args):
-    conv = [ctypes.c_void_p(a) if isinstance(a, int) and (a in P or a >= 1 << 50) else a for a in args]
+    conv = [ctypes.c_void_p(a) if isinstance(a, int) and (a - a % 4 in P or a >= 1 << 50) else a for a in args]
     return capi.lib().fn[name](*conv)
 
 
@@ -25,7 +25,7 @@ QUANT_OK = [0, P[0], 64, 100, 0, 1, 0, P[1], 112, P[2], P[3], 64, P[4]]
 
 @pytest.mark.parametrize("change", [
     dict(a=None), dict(rows=-1), dict(cols=-1), dict(format=2), dict(format=-1), dict(block_rows=64), dict(pow2=2), dict(q=None, qt=None), dict(scale=None), dict(scale_t=None),
-    dict(ldq=100), dict(ldq=96), dict(ldqt=48), dict(q=P[1] + 8), dict(qt=P[3] + 1), dict(q=P[0]), dict(qt=P[0] + 16), dict(qt=P[1]), dict(scale=P[1]), dict(scale_t=P[2])])
+    dict(ldq=100), dict(ldq=96), dict(ldqt=48), dict(q=P[1] + 8), dict(qt=P[3] + 1), dict(q=P[0]), dict(qt=P[0] + 16), dict(qt=P[1]), dict(scale=P[1]), dict(scale_t=P[2]), dict(a=P[0] + 2), dict(scale=P[2] + 1)])
 def test_quantize_refuses(change):
     assert call("fp8_quantize", with_changes(QUANT, QUANT_OK, change)) == INVAL
     assert "fp8_quantize" in capi.lib().last_error()
@@ -37,7 +37,7 @@ PROD_OK = [0, P[0], 112, P[1], 0, 1, P[2], 112, P[3], 1, 128, P[4], 0, 30, 40, 1
 
 @pytest.mark.parametrize("change", [
     dict(qa=None), dict(qb=None), dict(sa=None), dict(sb=None), dict(c=None), dict(fa=2), dict(fb=-1), dict(ba=2), dict(bb=0), dict(lda=96), dict(lda=100), dict(ldb=104), dict(ldb=1 << 40),
-    dict(qa=P[0] + 4), dict(qb=P[2] + 8), dict(m=-1), dict(n=-1), dict(k=-1), dict(c=P[0]), dict(c=P[2] + 64), dict(c=P[3])])
+    dict(qa=P[0] + 4), dict(qb=P[2] + 8), dict(m=-1), dict(n=-1), dict(k=-1), dict(c=P[0]), dict(c=P[2] + 64), dict(c=P[3]), dict(c=P[4] + 2), dict(sa=P[1] + 1)])
 def test_product_refuses(change):
     assert call("fp8_mult2d", with_changes(PROD, PROD_OK, change)) == INVAL
     assert "fp8_mult2d" in capi.lib().last_error()
@@ -51,7 +51,7 @@ NO_BLOCK = dict(f=None, r_out=None, gate=None, g1=None, b1=None, post=0, res_sca
 @pytest.mark.parametrize("change", [
     dict(kind=2), dict(post=2), dict(groups=-1), dict(rows=-1), dict(cols=0), dict(eps=-1.0), dict(eps=float("nan")), dict(r=None), dict(f=None), dict(r_out=None), dict(post=0), dict(post=0, g1=None), dict(h=None),
     dict(h=None, g2=None), dict(NO_BLOCK, res_scale=0.5), dict(NO_BLOCK, post=1), dict(NO_BLOCK, gate=P[2]), dict(NO_BLOCK, h=None, g2=None, b2=None), dict(stats=P[9] + 4), dict(r_out=P[1] + 4),
-    dict(r_out=P[2]), dict(r_out=P[8]), dict(h=P[5]), dict(h=P[0] + 400), dict(stats=P[0]), dict(stats=P[8])])
+    dict(r_out=P[2]), dict(r_out=P[8]), dict(h=P[5]), dict(h=P[0] + 400), dict(stats=P[0]), dict(stats=P[8]), dict(f=P[0] + 1), dict(h=P[8] + 2)])
 def test_norm_forward_refuses(change):
     assert call("norm_residual_fwd", with_changes(FWD, FWD_OK, change)) == INVAL
     assert "norm_residual_fwd" in capi.lib().last_error()
@@ -65,7 +65,7 @@ BWD_NO_BLOCK = dict(f=None, gate=None, g1=None, b1=None, post=0, res_scale=1.0, 
 @pytest.mark.parametrize("change", [
     dict(kind=-1), dict(post=3), dict(groups=-2), dict(rows=-1), dict(cols=0), dict(dh=None, dr_out=None), dict(dh=None), dict(dh=None, g2=None), dict(f=None), dict(BWD_NO_BLOCK, dgate=P[11]), dict(BWD_NO_BLOCK, df=P[9]),
     dict(BWD_NO_BLOCK, dg1=P[12]), dict(post=0), dict(post=0, g1=None, b1=None), dict(gate=None), dict(stats=None), dict(stats=P[8] + 8), dict(r_out=None), dict(df=P[0] + 4), dict(df=P[4]), dict(df=P[10]),
-    dict(dr=P[8]), dict(dr=P[0], inc_d=1), dict(df=P[2], inc_d=1), dict(dgate=P[0]), dict(dg1=P[5]), dict(dg2=P[12])])
+    dict(dr=P[8]), dict(dr=P[0], inc_d=1), dict(df=P[2], inc_d=1), dict(dgate=P[0]), dict(dg1=P[5]), dict(dg2=P[12]), dict(dh=P[0] + 2), dict(db2=P[15] + 1)])
 def test_norm_backward_refuses(change):
     assert call("norm_residual_bwd", with_changes(BWD, BWD_OK, change)) == INVAL
     assert "norm_residual_bwd" in capi.lib().last_error()
@@ -77,7 +77,7 @@ DIST_OK = [0, P[0], P[1], P[2], P[3], P[4], P[5], 6, 100, 104, 5, 2.0, 0.5, P[6]
 
 @pytest.mark.parametrize("change", [
     dict(logits=None), dict(ids=None), dict(teacher=None), dict(loss=None), dict(labels=None), dict(rows=-1), dict(cols=0), dict(ld=99), dict(k=0), dict(k=-1), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=1e-39),
-    dict(temperature=float("inf")), dict(temperature=float("nan")), dict(alpha=-0.1), dict(alpha=1.1), dict(alpha=float("nan")), dict(delta=P[0] + 4), dict(delta=P[1]), dict(loss=P[0]), dict(loss=P[7]), dict(loss=P[5])])
+    dict(temperature=float("inf")), dict(temperature=float("nan")), dict(alpha=-0.1), dict(alpha=1.1), dict(alpha=float("nan")), dict(delta=P[0] + 4), dict(delta=P[1]), dict(loss=P[0]), dict(loss=P[7]), dict(loss=P[5]), dict(logits=P[0] + 2), dict(ids=P[1] + 1)])
 def test_distill_refuses(change):
     assert call("distill", with_changes(DIST, DIST_OK, change)) == INVAL
     assert "distill" in capi.lib().last_error()
