@@ -252,14 +252,19 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, ProdShape<BN>::PER_SM)
     if (warp == 0) {
         // ============================ copies ============================
         if (elect_one()) {
-            int s = 0; uint32_t phase = 1;
-            for (int kb = kb0; kb < kb1; kb++) {
+            int s = 0, uses = 0; uint32_t phase = 1;
+            for (int kb = kb0; kb < kb1; kb++, uses++) {
                 if (!mbar_wait(bar_empty + 8 * s, phase, abort_flag)) { fail = 1; break; }
                 mbar_expect_tx(bar_full + 8 * s, S::STAGE);
                 const uint32_t dst = smem_u32(ring) + s * S::STAGE;
                 tma_load_2d(dst, &P.map_p, kb * kBlk, p0, bar_full + 8 * s);
                 tma_load_2d(dst + 128 * kBlk, &P.map_q, kb * kBlk, q0, bar_full + 8 * s);
                 if (++s == S::STAGES) { s = 0; phase ^= 1u; }
+            }
+            // no copy is on its way when the block ends, whoever gave up
+            for (int i = 0; i < S::STAGES && i < uses; i++) {
+                if (--s < 0) { s = S::STAGES - 1; phase ^= 1u; }
+                if (!mbar_wait(bar_full + 8 * s, phase ^ 1u, abort_flag)) fail = 5;
             }
         }
         __syncwarp();
@@ -470,9 +475,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
                 }
             }
             // the last arrivals on this CTA's barriers come from the other CTA: stay until they are in
-            for (int i = 0; i < LG_STAGES && i < uses && !fail; i++) {
+            // (after a wait that gave up: until the copies are in, which the first CTA's barriers know for both)
+            for (int i = 0; i < LG_STAGES && i < uses; i++) {
                 if (--s < 0) { s = LG_STAGES - 1; phase ^= 1u; }
-                if (!mbar_wait(bar_empty + 8 * s, phase ^ 1u, abort_flag)) fail = 5;
+                if (fail) { if (rank == 0) mbar_wait(bar_full + 8 * s, phase ^ 1u, abort_flag); }
+                else if (!mbar_wait(bar_empty + 8 * s, phase ^ 1u, abort_flag)) fail = 5;
             }
         } else if (warp == 1 && rank == 0 && elect_one()) {
             // ============================ MMA issue ============================
@@ -525,6 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
                 fetch(slot);
                 if (!mbar_wait(bar_acc_full + 8 * buf, phase, abort_flag)) fail = 4;
                 if (__any_sync(0xffffffffu, fail)) { fail = 4; return; }
+                if (VEC) __syncwarp();                       // the scales of the other lanes
                 tc_fence_after();
                 const uint32_t base = from + buf * 256;
                 uint32_t r[2][16];
@@ -653,7 +661,7 @@ int launch_product(DevCtx *cx, cudaStream_t st, const ProdParams &P, unsigned ti
 // the blocks divided by the size (1 x 6000 x 6000: 47 clusters of six are two rounds, 15.6 us, 47 of five one, 11.2).  Looked up with the first product on a
 // device, along with the kernels' attributes.  The query counts one block an SM of a kernel that uses tensor memory; two of the small tiles' are there
 // (10.3 warps of blocks of six active on an SM in a profile of 1 x 8192 x 8192), so its numbers of clusters are doubled.
-struct Residents { bool known = false; int of[5][9]; };
+struct Residents { bool known = false; int of[5][9]; };        // blocks, clusters of 2 .. 8
 Residents g_residents[EDDLB200_MAX_DEVICES];
 template <int BN>
 cudaError_t look_up_residents(int (&of)[9]) {

@@ -16,6 +16,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxCols = 16384;            // 1024 threads with four 16-byte pieces each; eight blocks of 256 with two each
 constexpr int kMaxCluster = 8;
+constexpr int kMaxRows = 0x7ff00000;       // of a group, and groups: counters that go past the last one stay in 32 bits
 
 // Sums of K values over a team of TPR threads (a warp, or the whole block); every thread gets them, added in a fixed order.  K is a power of two:
 // the lanes halve the number of values they carry with each of the first exchanges, so K sums of a warp cost K + 1 shuffles or so, not 5 K.
@@ -203,7 +204,7 @@ struct BwdArgs {
     float *df, *dr;
     float *param_part, *gate_part;          // [block][4][cols] of dg2, db2, dg1, db1; [unit][cols] of dgate, which is dgate itself where a unit is a group
     float res_scale;
-    int cols, chunk, rows, layer, post, inc_df, inc_dr; // chunk: columns of one block of a cluster;         // inc: 0 store, 1 add, 2 add to a destination known to hold zeros
+    int cols, chunk, rows, layer, post, inc_df, inc_dr; // chunk: columns of one block of a cluster; inc: 0 store, 1 add, 2 add to a destination known to hold zeros
     int want_gate, want_param, inc_gate;    // want_param: bits dg2, db2, dg1, db1; inc_gate: add to gate_part
     int unit_groups, slices, workers;       // a unit is a slice of a group's rows; workers: blocks (clusters) that share the units
     size_t unit_rows;                       // rows of one unit group
@@ -535,6 +536,7 @@ int eddlb200_norm_residual_fwd(int dev, int kind, int post, int groups, int rows
     EB_REQUIRE(groups >= 0 && rows >= 0 && cols > 0, kFwd);
     EB_REQUIRE(eps >= 0.f, kFwd);
     if (cols > kMaxCols) return set_error(EDDLB200_ELIMIT, "%s: rows of %d values, at most %d", kFwd, cols, kMaxCols);
+    if (groups > kMaxRows || rows > kMaxRows) return set_error(EDDLB200_ELIMIT, "%s: %d groups of %d rows", kFwd, groups, rows);
     EB_REQUIRE((f != nullptr) == (r_out != nullptr), kFwd);
     EB_REQUIRE(f || (!gate && !g1 && !b1 && !post && res_scale == 1.f), kFwd);
     EB_REQUIRE(post || (!g1 && !b1), kFwd);
@@ -578,6 +580,7 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
     EB_REQUIRE((kind == 0 || kind == 1) && (post == 0 || post == 1), kBwd);
     EB_REQUIRE(groups >= 0 && rows >= 0 && cols > 0, kBwd);
     if (cols > kMaxCols) return set_error(EDDLB200_ELIMIT, "%s: rows of %d values, at most %d", kBwd, cols, kMaxCols);
+    if (groups > kMaxRows || rows > kMaxRows) return set_error(EDDLB200_ELIMIT, "%s: %d groups of %d rows", kBwd, groups, rows);
     EB_REQUIRE(dh || dr_out, kBwd);
     EB_REQUIRE(dh || (!g2 && !dg2 && !db2), kBwd);
     EB_REQUIRE(f || (!gate && !g1 && !b1 && !post && res_scale == 1.f && !df), kBwd);
@@ -625,10 +628,12 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
     const bool fold = a.want_param || gate_floats;
     a.gate_part = dgate;
     a.inc_gate = dgate && !gate_floats && inc_g;
-    if (total && fold) {
+    if (total && (fold || dgate)) {
         cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
         if (int e = cuda_status(cudaStreamIsCapturing(st, &capturing), kBwd)) return e;
         if (capturing != cudaStreamCaptureStatusNone) return set_error(EDDLB200_EINVAL, "%s: the column sums use the library's scratch memory, which a captured graph must not hold", kBwd);
+    }
+    if (total && fold) {
         float *scr = (float *)scratch(cx, (param_floats + gate_floats) * sizeof(float));
         if (!scr) return cudaErrorMemoryAllocation;
         a.param_part = scr;

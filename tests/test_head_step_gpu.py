@@ -137,6 +137,8 @@ def test_captured_and_replayed(lib):
         H.forward()
         with pytest.raises(capi.Error, match="captured"):
             H.norm.backward(H.out, dh=H.dh)
+        with pytest.raises(capi.Error, match="captured"):
+            H.norm.backward({"dgate": H.out["dgate"]}, dh=H.dh)
         # without sums over rows nothing is kept: capturable
         H.norm.backward({k: H.out[k] for k in ("df", "dr")}, dh=H.dh)
     finally:

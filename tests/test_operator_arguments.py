@@ -86,6 +86,8 @@ def test_distill_refuses(change):
 def test_limits_are_told_apart_from_mistakes():
     assert call("norm_residual_fwd", with_changes(FWD, FWD_OK, dict(cols=16385))) == LIMIT
     assert call("norm_residual_bwd", with_changes(BWD, BWD_OK, dict(cols=16385))) == LIMIT
+    assert call("norm_residual_fwd", with_changes(FWD, FWD_OK, dict(rows=2 ** 31 - 1))) == LIMIT
+    assert call("norm_residual_bwd", with_changes(BWD, BWD_OK, dict(groups=2 ** 31 - 1))) == LIMIT
     assert call("distill", with_changes(DIST, DIST_OK, dict(cols=344065, ld=344065))) == LIMIT
     assert call("distill", with_changes(DIST, DIST_OK, dict(k=1025))) == LIMIT
     assert call("distill", with_changes(DIST, DIST_OK, dict(rows=2 ** 31 - 1, delta=None, loss=1 << 60))) == LIMIT
