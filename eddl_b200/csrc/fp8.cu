@@ -172,7 +172,7 @@ struct ProdParams {
     float *c;
     int p_rows, q_rows, kblocks;             // p_rows: columns of C, q_rows: rows of C
     int p_shift, q_shift, p_scales, q_scales;   // rows of a scale (log2) and scales of a K-block
-    int tiles_p, splits, inc;
+    int tiles_p, splits, inc, tail;          // tail: the kernel on pairs halves that many tiles, the last ones
     unsigned idesc;
 };
 
@@ -401,18 +401,26 @@ __device__ __forceinline__ void umma_fp8_pair(uint32_t d_tmem, uint64_t adesc, u
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// 16 columns of the warp's lanes, not waited for
-__device__ __forceinline__ void tmem_ask16(uint32_t taddr, uint32_t (&r)[16]) {
+// 16 or 8 columns of the warp's lanes, not waited for
+__device__ __forceinline__ void tmem_ask(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_ask(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+}
 // the registers of the loads so far may be read: they pass through the wait, so that no use of them is moved ahead of it
-__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) :: "memory");
 }
 __device__ __forceinline__ void sts(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ float lds(uint32_t addr) { float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory"); return v; }
@@ -420,7 +428,7 @@ __device__ __forceinline__ float4 lds4(uint32_t addr) {
     float4 v; asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory"); return v;
 }
 
-template <bool VEC, bool ROWS>
+template <bool VEC, bool ROWS, bool HALVES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_product_large_kernel(const __grid_constant__ ProdParams P) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -433,11 +441,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1), kblocks = P.kblocks;
-    const int tiles_p = P.tiles_p, tiles = tiles_p * P.splits;         // splits: here the tiles along Q
+    const int tiles_p = P.tiles_p, tail = HALVES ? P.tail : 0, whole = tiles_p * P.splits - tail, jobs = whole + 2 * tail;         // splits: here the tiles along Q
     // Tiles in bands of twelve along P, so that the pairs at work at a time share operands in L2 (8192 cubed: 600 us, in bands of eight 635).
-    auto place = [&](int tile, int &p0, int &q0) {
+    // The tiles of a last round that fills half of the pairs or less are worked on in halves of 128 rows of Q, job >= whole.
+    auto place = [&](int job, int &p0, int &q0) {
+        const int tile = !HALVES || job < whole ? job : whole + (job - whole) / 2;
         const int band = tile / (12 * P.splits), in = tile - band * 12 * P.splits, wide = min(12, tiles_p - band * 12);
-        p0 = (band * 12 + in % wide) * 256; q0 = in / wide * 256;
+        p0 = (band * 12 + in % wide) * 256; q0 = in / wide * 256 + (!HALVES || job < whole ? 0 : (job - whole) % 2 * 128);
     };
     if (threadIdx.x == 0) {
         for (int s = 0; s < LG_STAGES; s++) { mbar_init(bar_full + 8 * s, 1); mbar_init(bar_empty + 8 * s, 1); }
@@ -461,15 +471,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
             // ============================ copies ============================
             const uint32_t full_of_first = map_to_rank(bar_full, 0);
             int s = 0, uses = 0; uint32_t phase = 1;
-            for (int tile = pair; tile < tiles && !fail; tile += pairs) {
+            for (int job = pair; job < jobs && !fail; job += pairs) {
                 int p0, q0;
-                place(tile, p0, q0);
+                place(job, p0, q0);
+                const bool half = HALVES && job >= whole;
+                q0 += (int)rank * (half ? 64 : 128);
                 for (int kb = 0; kb < kblocks; kb++) {
                     if (!mbar_wait(bar_empty + 8 * s, phase, abort_flag)) { fail = 1; break; }
-                    if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * LG_STAGE);       // the bytes of both CTAs
+                    if (rank == 0) mbar_expect_tx(bar_full + 8 * s, half ? 2 * LG_STAGE - 128 * kBlk : 2 * LG_STAGE);       // the bytes of both CTAs
                     const uint32_t dst = smem_u32(ring) + s * LG_STAGE;
                     tma_load_2d_pair(dst, &P.map_p, kb * kBlk, p0 + (int)rank * 128, full_of_first + 8 * s);
-                    tma_load_2d_pair(dst + 128 * kBlk, &P.map_q, kb * kBlk, q0 + (int)rank * 128, full_of_first + 8 * s);
+                    tma_load_2d_pair(dst + 128 * kBlk, &P.map_q, kb * kBlk, q0, full_of_first + 8 * s);
+                    if (HALVES && !half) tma_load_2d_pair(dst + 192 * kBlk, &P.map_q, kb * kBlk, q0 + 64, full_of_first + 8 * s);
                     uses++;
                     if (++s == LG_STAGES) { s = 0; phase ^= 1u; }
                 }
@@ -484,92 +497,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
         } else if (warp == 1 && rank == 0 && elect_one()) {
             // ============================ MMA issue ============================
             int s = 0, buf = 0; uint32_t phase = 0, acc_phase = 1;
-            for (int tile = pair; tile < tiles && !fail; tile += pairs)
+            for (int job = pair; job < jobs && !fail; job += pairs) {
+                const unsigned idesc = !HALVES || job < whole ? P.idesc : P.idesc - (16u << 17);      // 256 or 128 columns
                 for (int kb = 0; kb < kblocks; kb++) {
                     if (!mbar_wait(bar_full + 8 * s, phase, abort_flag)) { fail = 3; break; }
                     if (!mbar_wait(bar_acc_empty + 8 * buf, acc_phase, abort_flag)) { fail = 2; break; }
                     tc_fence_after();
                     const uint64_t pd = make_desc(smem_u32(ring) + s * LG_STAGE), qd = make_desc(smem_u32(ring) + s * LG_STAGE + 128 * kBlk);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) umma_fp8_pair(tmem + buf * 256, pd + 2 * k, qd + 2 * k, P.idesc, k ? 1u : 0u);
+                    for (int k = 0; k < 4; k++) umma_fp8_pair(tmem + buf * 256, pd + 2 * k, qd + 2 * k, idesc, k ? 1u : 0u);
                     umma_commit_pair(bar_acc_full + 8 * buf);
                     umma_commit_pair(bar_empty + 8 * s);
                     if (++s == LG_STAGES) { s = 0; phase ^= 1u; }
                     if (++buf == 2) { buf = 0; acc_phase ^= 1u; }
                 }
+            }
         }
         __syncwarp();
     } else {
         // ============================ epilogue ============================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-        const int quarter = warp & 3, group = (warp - 4) >> 2;                 // 32 lanes, 64 columns
+        const int quarter = warp & 3, group = (warp - 4) >> 2;                 // 32 lanes, COLS columns
         const uint32_t empty_of_first = map_to_rank(bar_acc_empty, 0);
-        const uint32_t line = lines + (warp - 4) * LG_LINE, from = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * 64);
-        uint32_t buf = 0, phase = 0;
-        for (int tile = pair; tile < tiles; tile += pairs) {
+        const uint32_t line = lines + (warp - 4) * LG_LINE;
+        uint32_t done = 0;                                       // K-blocks: every other one lies in the first buffer
+        auto tile = [&](auto columns, int job) {
+            constexpr int COLS = decltype(columns)::value;
+            const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(group * COLS);
             int p0, q0;
-            place(tile, p0, q0);
-            const int p = p0 + (int)rank * 128 + quarter * 32 + lane, q = q0 + group * 64;
+            place(job, p0, q0);
+            const int p = p0 + (int)rank * 128 + quarter * 32 + lane, q = q0 + group * COLS;
             const float *sp = P.scale_p + (min(p, P.p_rows - 1) >> P.p_shift), *sq = P.scale_q + (VEC ? min(q + lane, P.q_rows - 1) : min(q, P.q_rows - 1) >> 7);
-            const int second = VEC && q + 32 + lane < P.q_rows ? 32 : 0;                // a column past the last one takes another's scale: its products are zero
-            float acc[64];
+            const int second = VEC && COLS == 64 && q + 32 + lane < P.q_rows ? 32 : 0;                // a column past the last one takes another's scale: its products are zero
+            float acc[COLS];
 #pragma unroll
-            for (int i = 0; i < 64; i++) acc[i] = 0.f;
+            for (int i = 0; i < COLS; i++) acc[i] = 0.f;
             // scales of the next two K-blocks, on their way
             float ahead_p[2], ahead_q[2][2];
             int left = kblocks;                              // K-blocks whose scales have not been asked for
-            auto fetch = [&](int slot) {
-                if (--left < 0) return;
+            auto fetch = [&](int slot, bool more) {
+                if (HALVES ? !more : --left < 0) return;     // the same; each form where it leaves no register spilled (with spills 8192 cubed took 800 us)
                 ahead_p[slot] = __ldg(sp);
                 ahead_q[slot][0] = __ldg(sq);
-                if (VEC) ahead_q[slot][1] = __ldg(sq + second);
+                if (VEC && COLS == 64) ahead_q[slot][1] = __ldg(sq + second);
                 sp += P.p_scales; sq += P.q_scales;
             };
-            auto block = [&](int slot) {
+            auto block = [&](int slot, bool more) {
                 const uint32_t scales = line + slot * 256;
                 const float s_p = VEC ? ahead_p[slot] : ahead_p[slot] * ahead_q[slot][0];
-                if (VEC) { sts(scales + lane * 4, ahead_q[slot][0]); sts(scales + 128 + lane * 4, ahead_q[slot][1]); }
-                fetch(slot);
-                if (!mbar_wait(bar_acc_full + 8 * buf, phase, abort_flag)) fail = 4;
+                if (VEC) sts(scales + lane * 4, ahead_q[slot][0]);
+                if (VEC && COLS == 64) sts(scales + 128 + lane * 4, ahead_q[slot][1]);
+                fetch(slot, more);
+                const uint32_t buf = done & 1;
+                if (!mbar_wait(bar_acc_full + 8 * buf, done >> 1 & 1, abort_flag)) fail = 4;
                 if (__any_sync(0xffffffffu, fail)) { fail = 4; return; }
                 if (VEC) __syncwarp();                       // the scales of the other lanes
                 tc_fence_after();
                 const uint32_t base = from + buf * 256;
-                uint32_t r[2][16];
-                tmem_ask16(base, r[0]);
+                constexpr int PIECE = VEC ? 8 : 16,                // the scales from shared memory take registers too (by 16 there: 120 us for 4096 cubed, by 8 110)
+                              PIECES = COLS / PIECE;
+                uint32_t r[2][PIECE];
+                tmem_ask(base, r[0]);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tmem_wait16(r[c & 1]);
-                    if (c < 3) tmem_ask16(base + 16 * (c + 1), r[(c + 1) & 1]);
+                for (int c = 0; c < PIECES; c++) {
+                    tmem_wait(r[c & 1]);
+                    if (c < PIECES - 1) tmem_ask(base + PIECE * (c + 1), r[(c + 1) & 1]);
                     else {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive_cluster(empty_of_first + 8 * buf);
                     }
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
+                    for (int j = 0; j < PIECE; j += 4) {
                         float4 d = make_float4(__uint_as_float(r[c & 1][j]), __uint_as_float(r[c & 1][j + 1]), __uint_as_float(r[c & 1][j + 2]), __uint_as_float(r[c & 1][j + 3]));
-                        if (VEC) { const float4 s4 = lds4(scales + (c * 16 + j) * 4); d.x *= s4.x; d.y *= s4.y; d.z *= s4.z; d.w *= s4.w; }
-                        float *to = acc + c * 16 + j;
+                        if (VEC) { const float4 s4 = lds4(scales + (c * PIECE + j) * 4); d.x *= s4.x; d.y *= s4.y; d.z *= s4.z; d.w *= s4.w; }
+                        float *to = acc + c * PIECE + j;
                         to[0] = fmaf(d.x, s_p, to[0]); to[1] = fmaf(d.y, s_p, to[1]); to[2] = fmaf(d.z, s_p, to[2]); to[3] = fmaf(d.w, s_p, to[3]);
                     }
                 }
-                buf ^= 1u;
-                if (!buf) phase ^= 1u;
+                done++;
             };
-            fetch(0); fetch(1);
+            fetch(0, true); fetch(1, kblocks > 1);
 #pragma unroll 1
             for (int kb = kblocks; kb > 0 && !fail; kb -= 2) {
-                block(0);
-                if (kb > 1 && !fail) block(1);
+                block(0, kb > 2);
+                if (kb > 1 && !fail) block(1, kb > 3);
             }
-            if (fail) break;
+            if (fail) return;
             if (ROWS) {
                 // C [p_rows][q_rows]: a lane holds a row's values, 32 rows x 16 columns at a time are turned
                 const int p_first = p0 + (int)rank * 128 + quarter * 32, rows = min(32, P.p_rows - p_first) - (lane >> 4);
                 auto out = [&](auto whole, auto inc) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
+                    for (int c = 0; c < COLS / 16; c++) {
                         __syncwarp();
 #pragma unroll
                         for (int j = 0; j < 16; j++) sts(line + (lane * 17 + j) * 4, acc[c * 16 + j]);
@@ -593,14 +613,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
                 // C [q_rows][p_rows]: the lanes are neighbours in memory
                 float *dst = P.c + (size_t)q * P.p_rows + p;
                 const int columns = P.q_rows - q;
-                if (!P.inc && columns >= 64) {
+                if (!P.inc && columns >= COLS) {
 #pragma unroll
-                    for (int i = 0; i < 64; i++, dst += P.p_rows) *dst = acc[i];
+                    for (int i = 0; i < COLS; i++, dst += P.p_rows) *dst = acc[i];
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 64; i++, dst += P.p_rows) if (i < columns) *dst = P.inc ? *dst + acc[i] : acc[i];
+                    for (int i = 0; i < COLS; i++, dst += P.p_rows) if (i < columns) *dst = P.inc ? *dst + acc[i] : acc[i];
                 }
             }
+        };
+        for (int job = pair; job < jobs && !fail; job += pairs) {
+            if (!HALVES || job < whole) tile(std::integral_constant<int, 64>(), job);
+            else if constexpr (HALVES) tile(std::integral_constant<int, 32>(), job);
         }
     }
     if (fail) { *abort_flag = 1; atomicCAS(&g_fp8_status, 0, fail | warp << 8 | 7 << 16); }
@@ -611,19 +635,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
     if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-template <bool VEC, bool ROWS>
+template <bool VEC, bool ROWS, bool HALVES>
 int launch_large(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P) {
     static bool configured[EDDLB200_MAX_DEVICES] = {};
     if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(fp8_product_large_kernel<VEC, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(fp8_product_large_kernel<VEC, ROWS, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SMEM);
         if (e != cudaSuccess) return cuda_status(e, "fp8_mult2d(attributes)");
         configured[dev] = true;
     }
-    const int tiles = P.tiles_p * P.splits, pairs = tiles < EDDLB200_NUM_SMS / 2 ? tiles : EDDLB200_NUM_SMS / 2;
-    eb::launch(fp8_product_large_kernel<VEC, ROWS>, 2 * pairs, LG_THREADS, LG_SMEM, st, P);
+    const int jobs = P.tiles_p * P.splits + P.tail, pairs = jobs < EDDLB200_NUM_SMS / 2 ? jobs : EDDLB200_NUM_SMS / 2;
+    eb::launch(fp8_product_large_kernel<VEC, ROWS, HALVES>, 2 * pairs, LG_THREADS, LG_SMEM, st, P);
     EB_LAUNCH_CHECK("fp8_mult2d");
     g_fp8_used[dev] = true;
     return 0;
+}
+
+template <bool HALVES>
+int large_product(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P, int block_a, int block_b) {
+    return block_b == kBlk ? launch_large<false, true, HALVES>(cx, dev, st, P) : block_a == kBlk ? launch_large<false, false, HALVES>(cx, dev, st, P) : launch_large<true, false, HALVES>(cx, dev, st, P);
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
@@ -698,11 +727,16 @@ int product_residents(int dev, const Residents *&out) {
 // 1024 x 4096 x 4096 over all tiles and splits; the estimates are within 20 % of it.  A K-block costs an SM its operands' way through L2 or, in the
 // wide tiles, the epilogue's; alone on its SM a block waits at least for its own chain.  A tile costs its start and its stores and, when split,
 // the exchange between the blocks of a cluster.  256 x 4096 x 4096: 128 rows in two splits 15.8 us, pairs 22.0; 2048 cubed: pairs 16.0, 256 rows 24.8.
-struct Plan { int bn = 0, splits = 1; size_t tiles = 0; };           // bn 0: the kernel on pairs of CTAs
+struct Plan { int bn = 0, splits = 1; size_t tiles = 0, halved = 0; };   // bn 0: the kernel on pairs of CTAs, which halves the last tiles
 Plan pick_plan(const Residents &held, int m, int n, int kblocks) {
     Plan best;
     best.tiles = ceil_div(m, 256) * ceil_div(n, 256);
-    double least = (double)ceil_div(best.tiles, (size_t)EDDLB200_NUM_SMS / 2) * (1050.0 * kblocks + 8000.0);
+    // a last round for half of the pairs or less is halved (2304 x 2304 x 4096: 52 us, in two whole rounds 63; 4096 cubed 90 and 94; 512 x 4096 x 4096:
+    // 17.9, with tiles of 256 x 128 on single CTAs 26)
+    const size_t pairs = EDDLB200_NUM_SMS / 2, last = best.tiles % pairs;
+    best.halved = last <= pairs / 2 ? last : 0;
+    const double last_block = last > pairs / 2 ? 1050.0 : last ? 630.0 : 0.0;
+    double least = (best.tiles / pairs * 1050.0 + last_block) * kblocks + (double)ceil_div(best.tiles, pairs) * 8000.0;
     for (int bn = 16; bn <= 256; bn *= 2) {
         if (bn > 16 && bn / 2 >= m) break;                           // half of the tile would be empty
         const int which = bn == 16 ? 0 : bn == 32 ? 1 : bn == 64 ? 2 : bn == 128 ? 3 : 4;
@@ -817,8 +851,9 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
         if (plan.tiles > 0x0fffffff) return set_error(EDDLB200_ELIMIT, "%s: %d x %d", what, m, n);
         // C's rows are P's where only B's scales are shared by 128 rows: the side whose scales cost less is Q (see the kernel on pairs)
         const bool rows = !plan.bn && block_b == kBlk;
-        if (!(plan.bn ? sides(sb, sa, 128, plan.bn) : rows ? sides(sa, sb, 128, 128) : sides(sb, sa, 128, 128)))
-            return set_error(EDDLB200_EINVAL, "%s: the driver refuses a tensor map of the operands", what);
+        P.tail = plan.bn ? 0 : (int)plan.halved;
+        const int p_box = 128, q_box = plan.bn ? plan.bn : P.tail ? 64 : 128;
+        if (!(rows ? sides(sa, sb, p_box, q_box) : sides(sb, sa, p_box, q_box))) return set_error(EDDLB200_EINVAL, "%s: the driver refuses a tensor map of the operands", what);
         P.tiles_p = (int)ceil_div(P.p_rows, plan.bn ? 128 : 256);
         P.splits = plan.bn ? plan.splits : (int)ceil_div(P.q_rows, 256);
         const int m_side = plan.bn ? 128 : 256, n_side = plan.bn ? plan.bn : 256;
@@ -837,7 +872,7 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     if (!k) return inc_c ? 0 : launch_zero_fill(cx, st, c, (size_t)m * n);
     g_fp8_used[dev] = true;
     if (!plan.bn)
-        return block_b == kBlk ? launch_large<false, true>(cx, dev, st, P) : block_a == kBlk ? launch_large<false, false>(cx, dev, st, P) : launch_large<true, false>(cx, dev, st, P);
+        return P.tail ? large_product<true>(cx, dev, st, P, block_a, block_b) : large_product<false>(cx, dev, st, P, block_a, block_b);
     switch (plan.bn) {
         case 16: return launch_product<16>(cx, st, P, (unsigned)plan.tiles);
         case 32: return launch_product<32>(cx, st, P, (unsigned)plan.tiles);

@@ -183,7 +183,7 @@ def test_product(lib, m, n, k, blocks, inc):
 
 
 # many tiles of 256 x 256: whole and ragged ones, one and several rounds of them, few and many K-blocks, an odd number of them
-@pytest.mark.parametrize("m,n,k", [(1537, 1601, 260), (300, 9601, 700), (9999, 130, 513), (2048, 1536, 128), (4096, 4352, 64), (1600, 1700, 2000)])
+@pytest.mark.parametrize("m,n,k", [(1537, 1601, 260), (300, 9601, 700), (9999, 130, 513), (2048, 1536, 128), (4096, 4352, 64), (1600, 1700, 2000), (2500, 2300, 300), (2100, 2400, 140), (2400, 2100, 140), (4096, 2304, 384)])
 @pytest.mark.parametrize("blocks", [(1, 128), (1, 1), (128, 128), (128, 1)])
 @pytest.mark.parametrize("inc", [0, 1])
 def test_large_product(lib, m, n, k, blocks, inc):
