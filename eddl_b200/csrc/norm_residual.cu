@@ -123,12 +123,14 @@ struct FwdArgs {
     size_t total;
 };
 
-template <int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_fwd_kernel(const FwdArgs a) {
+template <int TPR, int NV, bool VEC, bool AHEAD>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 512 && AHEAD ? 2 : TPR == 256 ? 3 : 1) norm_residual_fwd_kernel(const FwdArgs a) {
     EB_GRID_WAIT();
+    extern __shared__ __align__(16) float staged[];                    // AHEAD: [team][r, f][SPAN]
     __shared__ float sums[2 * (TPR / 32)];
     TeamSum<TPR, 1> sum(sums);
-    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4;
+    constexpr int TEAMS = TPR == 32 ? 8 : 1, N = NV * 4, SPAN = TPR * N;
+    static_assert(VEC || !AHEAD, "");
     const Piece<TPR, NV, VEC> piece{(int)(threadIdx.x % TPR), a.cols};
     const float inv = 1.f / (float)a.cols;
     // mean and 1 / deviation of the team's row; the values are centred in place
@@ -151,13 +153,32 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR) norm_residual_fwd_kerne
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] *= rstd;
     };
-    for (size_t row = (size_t)blockIdx.x * TEAMS + threadIdx.x / TPR; row < a.total; row += (size_t)gridDim.x * TEAMS) {
+    float *own = staged + (size_t)(threadIdx.x / TPR) * (2 * SPAN);
+    const size_t first = (size_t)blockIdx.x * TEAMS + threadIdx.x / TPR, step = (size_t)gridDim.x * TEAMS;
+    auto ask = [&](size_t row) {
+        if (row < a.total) {
+            const size_t base = row * a.cols;
+            piece.ask(own, a.r + base);
+            if (a.f) piece.ask(own + SPAN, a.f + base);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (AHEAD) ask(first);
+    for (size_t row = first; row < a.total; row += step) {
         float v[N], x[N];
         float mean1 = 0.f, rstd1 = 0.f, mean2 = 0.f, rstd2 = 0.f;
         const size_t base = row * a.cols;
-        piece.load(x, a.r + base, 0.f);
+        if (AHEAD) {
+            // a thread reads what it copied itself, and its places are free again once the values are in registers
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            piece.load(x, own, 0.f);
+            if (a.f) piece.load(v, own + SPAN, 0.f);
+            ask(row + step);
+        } else {
+            piece.load(x, a.r + base, 0.f);
+            if (a.f) piece.load(v, a.f + base, 0.f);
+        }
         if (a.f) {
-            piece.load(v, a.f + base, 0.f);
             if (a.post) normalise(v, mean1, rstd1);
             float p[N];
             if (a.g1) {
@@ -462,12 +483,36 @@ __global__ void __launch_bounds__(1024) norm_residual_fold_kernel(const FoldArgs
 }
 
 template <int TPR, int NV>
-void launch_fwd(cudaStream_t st, const FwdArgs &a, bool vec) {
-    constexpr int block = TPR == 32 ? 256 : TPR, teams = TPR == 32 ? 8 : 1;
-    const size_t want = ceil_div(a.total, teams), most = (size_t)EDDLB200_NUM_SMS * (2048 / block);
-    const unsigned grid = (unsigned)(want < most ? want : most);
-    eb::launch(vec ? norm_residual_fwd_kernel<TPR, NV, true> : norm_residual_fwd_kernel<TPR, NV, false>, grid, block, 0, st, a);
-}
+struct Fwd {
+    // Aligned rows are copied ahead where few blocks share an SM (8192 columns, 4000 rows: 89 us, without 111) or rows are short (128 columns, 100000 rows:
+    // 45 us, without 51), not in between (4096 columns, 12288 rows: 142 us, without 132): there the blocks of an SM cover for one another.
+    static constexpr bool AHEAD = TPR * NV > 1024 || (TPR == 32 && NV == 1);
+    static int run(DevCtx *cx, int dev, cudaStream_t st, const FwdArgs &a, bool vec) {
+        constexpr int block = TPR == 32 ? 256 : TPR, teams = TPR == 32 ? 8 : 1;
+        const size_t want = ceil_div(a.total, teams), most = (size_t)EDDLB200_NUM_SMS * (2048 / block);
+        if constexpr (AHEAD) if (vec) {
+            constexpr size_t smem = (size_t)teams * 2 * TPR * NV * 4 * sizeof(float);
+            static int known[EDDLB200_MAX_DEVICES] = {};                       // blocks that the device holds at once
+            int &n = known[dev];
+            auto kernel = norm_residual_fwd_kernel<TPR, NV, true, true>;
+            if (!n) {
+                cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                int held = 0;
+                if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, block, smem);
+                if (e != cudaSuccess) return cuda_status(e, "norm_residual_fwd(occupancy)");
+                n = (held < 1 ? 1 : held) * EDDLB200_NUM_SMS;
+            }
+            if (want > (size_t)n) {
+                eb::launch(kernel, (unsigned)n, block, smem, st, a);
+                EB_LAUNCH_CHECK("norm_residual_fwd");
+                return 0;
+            }
+        }
+        eb::launch(vec ? norm_residual_fwd_kernel<TPR, NV, true, false> : norm_residual_fwd_kernel<TPR, NV, false, false>, (unsigned)(want < most ? want : most), block, 0, st, a);
+        EB_LAUNCH_CHECK("norm_residual_fwd");
+        return 0;
+    }
+};
 
 template <int TPR, int NV, bool CLUSTER>
 struct Bwd {
@@ -506,14 +551,18 @@ struct Bwd {
         return 0;
     }
 };
-// The smallest team that holds a row in registers beside its column sums: eight values a thread at most; wider rows are shared by a cluster.
+// The smallest team that holds a row in registers beside its column sums: eight values a thread at most; wider rows are shared by a cluster.  Teams between
+// the powers of two where half of the lanes would be idle (10000 x 1300, layer norms: 69 us on 192 threads, 83 on 256; 6000 x 2500: 85 on 320, 112 on 512).
 template <typename Go>
 auto with_bwd(int cols, Go go) {
     if (cols <= 128) return go(Bwd<32, 1, false>());
     if (cols <= 256) return go(Bwd<32, 2, false>());
     if (cols <= 512) return go(Bwd<128, 1, false>());
+    if (cols <= 768) return go(Bwd<96, 2, false>());
     if (cols <= 1024) return go(Bwd<128, 2, false>());
+    if (cols <= 1536) return go(Bwd<192, 2, false>());
     if (cols <= 2048) return go(Bwd<256, 2, false>());
+    if (cols <= 2560) return go(Bwd<320, 2, false>());
     if (cols <= 4096) return go(Bwd<512, 2, false>());
     return go(Bwd<256, 2, true>());
 }
@@ -562,16 +611,22 @@ int eddlb200_norm_residual_fwd(int dev, int kind, int post, int groups, int rows
     const FwdArgs a{f, r, gate, g1, b1, g2, b2, r_out, h, stats, res_scale, eps, cols, rows, kind, post, total};
     const bool vec = cols % 4 == 0 && aligned16(f) && aligned16(r) && aligned16(gate) && aligned16(g1) && aligned16(b1) && aligned16(g2) && aligned16(b2) && aligned16(r_out) && aligned16(h);
     const bool few = total < (size_t)EDDLB200_NUM_SMS * 8;          // rows for one warp a scheduler or less: several warps a row
-    if (cols <= 128) launch_fwd<32, 1>(st, a, vec);
-    else if (cols <= 256) launch_fwd<32, 2>(st, a, vec);
-    else if (cols <= 512) { if (few) launch_fwd<128, 1>(st, a, vec); else launch_fwd<32, 4>(st, a, vec); }
-    else if (cols <= 1024) { if (few) launch_fwd<128, 2>(st, a, vec); else launch_fwd<32, 8>(st, a, vec); }
-    else if (cols <= 2048) launch_fwd<256, 2>(st, a, vec);
-    else if (cols <= 4096) launch_fwd<512, 2>(st, a, vec);
-    else if (cols <= 8192) launch_fwd<1024, 2>(st, a, vec);
-    else launch_fwd<1024, 4>(st, a, vec);
-    EB_LAUNCH_CHECK(kFwd);
-    return 0;
+    // Twelve to 32 values a thread: a row on fewer threads means fewer to add up and to wait for, and idle lanes cost as much as others (10000 x 1300,
+    // layer norms: 44 us on 128 threads, 61 on 256; 12288 x 4096: 132 on 256, 142 on 512; 12544 x 768: 29 on 64, 31 on 32; 6000 x 2400: 41 on 128,
+    // 49 on 256; 3000 x 6000: 53 on 512 with 12 values, 55 on 384 with 16).
+    auto go = [&](auto k) { return decltype(k)::run(cx, dev, st, a, vec); };
+    if (cols <= 128) return go(Fwd<32, 1>());
+    if (cols <= 256) return go(Fwd<32, 2>());
+    if (cols <= 512) return few ? go(Fwd<128, 1>()) : go(Fwd<32, 4>());
+    if (cols <= 768) return few ? go(Fwd<128, 2>()) : go(Fwd<64, 3>());
+    if (cols <= 1024) return few ? go(Fwd<128, 2>()) : go(Fwd<32, 8>());
+    if (cols <= 1536) return go(Fwd<128, 3>());
+    if (cols <= 2048) return go(Fwd<64, 8>());
+    if (cols <= 2560) return go(Fwd<128, 5>());
+    if (cols <= 4096) return go(Fwd<256, 4>());
+    if (cols <= 6144) return go(Fwd<512, 3>());
+    if (cols <= 8192) return go(Fwd<512, 4>());
+    return go(Fwd<1024, 4>());
 }
 
 int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows, int cols, const float *dh, const float *dr_out, const float *f,

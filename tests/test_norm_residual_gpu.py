@@ -146,7 +146,8 @@ def check(lib, c, dh=True, dr_out=True, inc_d=0, inc_g=0):
 
 
 SHAPES = [(1, 1, 1), (1, 3, 5), (2, 7, 64), (3, 5, 127), (1, 40, 128), (5, 9, 130), (2, 33, 256), (7, 1, 257), (2, 30, 512), (3, 4, 771), (1, 9, 1024), (2, 6, 1028), (4, 3, 2048),
-          (1, 5, 2049), (2, 3, 4096), (1, 3, 4100), (2, 2, 5001), (1, 2, 8192), (1, 3, 12000), (1, 2, 16384), (1, 3, 16383), (300, 2, 32), (2, 700, 96), (1, 3000, 260)]
+          (1, 5, 2049), (2, 3, 4096), (1, 3, 4100), (2, 2, 5001), (1, 2, 8192), (1, 3, 12000), (1, 2, 16384), (1, 3, 16383), (300, 2, 32), (2, 700, 96), (1, 3000, 260),
+          (1, 13000, 100), (1, 1300, 700), (1, 1301, 701), (2, 50, 1400), (1, 60, 1535), (2, 41, 2304), (1, 40, 2303), (1, 500, 4352), (2, 300, 6148), (1, 350, 8192), (1, 200, 12004)]
 
 
 @pytest.mark.parametrize("dims", SHAPES)
