@@ -46,7 +46,7 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 __device__ __forceinline__ float exp2_fast(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
 constexpr float kLog2e = 1.44269504f;
 // exp(d) beside `e`, exp(d / T): an exponential of its own, or e^T for the temperatures 2 and 4, the usual ones (four exponentials of a logit are
-// half of the 222 us that 4096 x 32000 takes at 16 a cycle and SM)
+// 110 us of 4096 x 32000 at 16 a cycle and SM: 222 us with them, 205 with two)
 enum : int { kNoExp, kOwnExp, kSquare, kFourth };
 template <int HOW> struct Exp { static constexpr int value = HOW; };
 template <int HOW>
