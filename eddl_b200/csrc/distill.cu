@@ -462,43 +462,48 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
     if (CLUSTER) cg::this_cluster().sync();                // a block's lines outlive the writes of the others
 }
 
+constexpr size_t kSmemSM = 227 * 1024, kStatic = 4 * 1024;             // of an SM; what a block takes beside its own
+int blocks_held(size_t smem, int team) {
+    const size_t n = kSmemSM / (smem + kStatic);
+    return (int)(n < 1 ? 1 : n > (size_t)blocks_per_sm(team) ? (size_t)blocks_per_sm(team) : n);
+}
 template <int TEAM, bool CLUSTER>
-int launch_distill(DevCtx *cx, int dev, cudaStream_t st, const Args &a, unsigned csize, size_t smem) {
+int set_attributes(int dev) {
     static bool configured[EDDLB200_MAX_DEVICES] = {};
-    auto kernel = distill_kernel<TEAM, CLUSTER>;
-    if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
-        if (e != cudaSuccess) return cuda_status(e, "distill(attributes)");
-        configured[dev] = true;
-    }
-    constexpr int block = block_of(TEAM, CLUSTER), teams = TEAM == 32 ? 8 : 1;
-    size_t per_sm = (size_t)227 * 1024 / (smem + 4 * 1024);
-    if (per_sm > (size_t)blocks_per_sm(TEAM)) per_sm = blocks_per_sm(TEAM);
-    if (per_sm < 1) per_sm = 1;
-    size_t most = EDDLB200_NUM_SMS * per_sm / csize;
-    if (CLUSTER) {
-        // The blocks of a cluster share a group of SMs, whose number need not divide by what they take: with more clusters than the GPU holds
-        // at once the rows of the last ones would wait for a whole round (1023 x 131071, 55 clusters of which 48 fit: 434 us, with 48 below).
-        static struct { size_t smem; int clusters; } held[EDDLB200_MAX_DEVICES][kMaxCluster + 1] = {};
-        auto &h = held[dev][csize];
-        if (h.smem != smem) {
-            cudaLaunchAttribute at[1];
-            at[0].id = cudaLaunchAttributeClusterDimension; at[0].val.clusterDim.x = csize; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-            cudaLaunchConfig_t c = {};
-            c.gridDim = dim3((unsigned)(most * csize)); c.blockDim = dim3(block); c.dynamicSmemBytes = smem; c.attrs = at; c.numAttrs = 1;
-            int clusters = 0;
-            const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &c);
-            if (e != cudaSuccess) return cuda_status(e, "distill(clusters)");
-            h.smem = smem; h.clusters = clusters;
-        }
-        if ((size_t)h.clusters < most) most = h.clusters;
-        if (most < 1) return set_error(EDDLB200_ELIMIT, "distill: the device holds no cluster of %u blocks with %zu bytes each", csize, smem);
-    }
-    const size_t want = ceil_div(a.rows, teams);
-    const unsigned clusters = (unsigned)(want < most ? want : most);
-    if (CLUSTER) eb::launch_cluster(kernel, csize, clusters * csize, block, smem, st, a);
-    else eb::launch(kernel, clusters, block, smem, st, a);
+    if (configured[dev]) return 0;
+    const cudaError_t e = cudaFuncSetAttribute(distill_kernel<TEAM, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
+    if (e != cudaSuccess) return cuda_status(e, "distill(attributes)");
+    configured[dev] = true;
+    return 0;
+}
+template <int TEAM>
+int launch_distill(DevCtx *cx, int dev, cudaStream_t st, const Args &a, size_t smem) {
+    if (int e = set_attributes<TEAM, false>(dev)) return e;
+    const size_t want = ceil_div(a.rows, TEAM == 32 ? 8 : 1), most = (size_t)EDDLB200_NUM_SMS * blocks_held(smem, TEAM);
+    eb::launch(distill_kernel<TEAM, false>, (unsigned)(want < most ? want : most), block_of(TEAM, false), smem, st, a);
     EB_LAUNCH_CHECK("distill");
+    return 0;
+}
+// Clusters of `csize` blocks, `per_sm` of which fit an SM, that the device holds at once.  The blocks of a cluster share a group of SMs, whose number need
+// not divide by what they take: with more clusters than the GPU holds the rows of the last ones would wait for a whole round (1023 x 131071,
+// 55 clusters of eight of which 48 fit: 434 us, with 48 252).
+int clusters_held(int dev, int csize, int per_sm, int &out) {
+    static int known[EDDLB200_MAX_DEVICES][kMaxCluster + 1][4] = {};
+    int &n = known[dev][csize][per_sm];
+    if (!n) {
+        if (int e = set_attributes<256, true>(dev)) return e;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension; at[0].val.clusterDim.x = csize; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t c = {};
+        c.gridDim = dim3((unsigned)(EDDLB200_NUM_SMS * per_sm / csize * csize)); c.blockDim = dim3(block_of(256, true));
+        c.dynamicSmemBytes = kSmemSM / per_sm - kStatic; c.attrs = at; c.numAttrs = 1;
+        if (c.dynamicSmemBytes > 222 * 1024) c.dynamicSmemBytes = 222 * 1024;
+        int held = 0;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&held, distill_kernel<256, true>, &c);
+        if (e != cudaSuccess) return cuda_status(e, "distill(clusters)");
+        n = held < 1 ? -1 : held;
+    }
+    out = n < 0 ? 0 : n;
     return 0;
 }
 
@@ -538,10 +543,29 @@ extern "C" int eddlb200_distill(int dev, const float *logits, const int *ids, co
     auto smem = [&](unsigned c, int records) { a.piece = (int)((ceil_div(cols, c) + 3) & ~(size_t)3); return ((size_t)a.piece + 4 + 3 * records * kk) * sizeof(float); };
     // A warp a row, entries and all, as long as two blocks of eight rows fit an SM and there are rows for every SM: nothing waits for anything but its own
     // latencies (40000 x 1300, 32 entries: 119 us, with a block a row 233; 16384 x 4000, where one block fits: 180 and 147).
-    if (cols <= 256 || (8 * smem(1, 1) <= 112 * 1024 && rows >= EDDLB200_NUM_SMS * 8)) { const size_t b = 8 * smem(1, 1); return launch_distill<32, false>(cx, dev, st, a, 1, b); }
-    if (cols <= 8192) { const size_t b = smem(1, 4); return launch_distill<128, false>(cx, dev, st, a, 1, b); }
-    if (cols <= 16384) { const size_t b = smem(1, 4); return launch_distill<256, false>(cx, dev, st, a, 1, b); }
-    const unsigned csize = cols <= 32768 ? 2 : cols <= 65536 ? 4 : 8;
+    if (cols <= 256 || (8 * smem(1, 1) <= 112 * 1024 && rows >= EDDLB200_NUM_SMS * 8)) { const size_t b = 8 * smem(1, 1); return launch_distill<32>(cx, dev, st, a, b); }
+    if (cols <= 8192) { const size_t b = smem(1, 4); return launch_distill<128>(cx, dev, st, a, b); }
+    if (cols <= 16384) { const size_t b = smem(1, 4); return launch_distill<256>(cx, dev, st, a, b); }
+    // A cluster's size: the least of rounds x time of a round, 3.6 us and 0.21, 0.35 or 0.48 ns a logit of a block with one, two or three of them on its SM,
+    // or the look-up of many entries if that is longer (within 8 % of 50 measured pairs of shape and size).  1023 x 131071: five blocks 241 us,
+    // eight 252, four 286; 1000 x 80000: five 137, eight 165; 2000 x 50257: three 163, four 176; 4096 x 32000: two 208, three 242.
+    unsigned csize = 0, clusters = 0;
+    double least = 0.0;
+    for (int c = kMaxCluster; c >= 2; c--) {
+        const size_t b = smem(c, 3);
+        if (a.piece > kMaxPiece) break;
+        const int per_sm = blocks_held(b, 256);
+        int held = 0;
+        if (int e = clusters_held(dev, c, per_sm, held)) return e;
+        if (!held) continue;
+        const int at_once = rows < held ? rows : held, full = (int)ceil_div((size_t)at_once * c, (size_t)EDDLB200_NUM_SMS), on_sm = full < per_sm ? full : per_sm;
+        const double round = 3570.0 + a.piece * (on_sm == 1 ? 0.21 : on_sm == 2 ? 0.35 : 0.48), look = 0.09 * k * k;
+        const double t = (double)ceil_div(rows, held) * (round > look ? round : look);
+        if (!csize || t < least) { csize = c; clusters = at_once; least = t; }
+    }
+    if (!csize) return set_error(EDDLB200_ELIMIT, "%s: the device holds no cluster for rows of %d classes", what, cols);
     const size_t b = smem(csize, 3);
-    return launch_distill<256, true>(cx, dev, st, a, csize, b);
+    eb::launch_cluster(distill_kernel<256, true>, csize, clusters * csize, block_of(256, true), b, st, a);
+    EB_LAUNCH_CHECK(what);
+    return 0;
 }
