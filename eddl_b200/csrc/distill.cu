@@ -54,12 +54,14 @@ __device__ __forceinline__ float plain(float d, float e) { return HOW == kSquare
 
 // What a row's entries and its label add.  loss = base + per_z ((m - anchor) / T + ln z) - per_rest (ln z_out - ln z) + hard (m - x_label + ln z_1), with
 // m the row's largest logit, z and z_1 the sums of exp((x - m) / T) and exp(x - m), z_out the first one outside the entries; the gradient is
-// inside / z - rest / z_out times the exponential outside the entries, inside / z times it minus `less` at an entry.
+// inside / z - rest / z_out times the exponential outside the entries, inside / z times it minus `less` at an entry.  Where the entries hold less than half
+// of the student's mass, z_in / z, the logarithm of z_out / z and that difference come from z_in / z: (entries - inside z_in / z) / z_out; what is
+// left of them after subtracting numbers near 1 would be good to a few digits only.
 struct Head {
     double base, per_z, per_rest, hard;
-    float inside, rest, x_label, anchor;         // anchor: the largest of the entries' logits
+    float inside, rest, entries, x_label, anchor;         // anchor: the largest of the entries' logits
     float z, z1;                                 // the entries' sums relative to it, where their cells are closed
-    float row_m, row_out, row_z, row_z1;         // what the other warps found of the row: m, z_out, z, z_1; m = -infinity: nothing that counts
+    float row_m, row_in, row_out, row_z, row_z1;         // what the other warps found of the row: m, z_in, z_out, z, z_1; m = -infinity: nothing that counts
     int label, label_is_entry, live;
 };
 struct Record {
@@ -177,11 +179,12 @@ __device__ void look_up(const Args &a, int row, int next_row, Ahead &ahead, cons
         const double rest = tail && entries ? fmax(0.0, 1.0 - sum) : 0.0, wt = ws * a.temperature;
         Head h;
         h.hard = label >= 0 ? (double)weight * a.alpha : 0.0;
-        h.base = entries ? wt * (tail ? terms + (rest > 0.0 ? rest * logf((float)rest) : 0.0) : terms * per_sum - logf((float)sum)) : 0.0;
+        h.base = entries ? wt * (tail ? terms + (rest > 0.0 ? rest * (sum < 0.5 ? log1pf((float)-sum) : logf((float)rest)) : 0.0) : terms * per_sum - logf((float)sum)) : 0.0;
         h.per_z = entries ? wt * (tail ? sum : 1.0) : 0.0;
         h.per_rest = wt * rest;
         h.inside = (float)(ws * (tail ? sum + rest : 1.0));
         h.rest = (float)(ws * rest);
+        h.entries = (float)(ws * sum);
         h.x_label = x_label; h.anchor = anchor; h.z = z; h.z1 = z1;
         h.label = label; h.label_is_entry = label_seen; h.live = 1;
         *r.head = h;
@@ -257,10 +260,10 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
         run.meet(top, c_t); own.meet(top, c_t);
         return own;
     };
-    auto loss_of = [&](const Head &h, float m, float z_out, float z, float z1) {
+    auto loss_of = [&](const Head &h, float m, float z_in, float z_out, float z, float z1) {
         double l = h.base;
         if (any_entries) l += h.per_z * (((double)m - (double)h.anchor) / (double)a.temperature + (double)logf(z));
-        if (h.per_rest > 0.0) l -= h.per_rest * ((double)logf(z_out) - (double)logf(z));
+        if (h.per_rest > 0.0) l -= h.per_rest * (double)(z_in < 0.5f * z ? log1pf(-z_in / z) : logf(z_out / z));
         if (h.label >= 0) l += h.hard * ((double)m - (double)h.x_label + (double)logf(z1));
         return (float)l;
     };
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
                     Run run = combine(flip);
                     const Run own = add_entries(run, h);
                     const float z = run.z + own.z;
-                    if (run.m != minus_inf()) loss = loss_of(h, run.m, run.z, z, one_exp && any_entries ? z : run.z1 + own.z1);
+                    if (run.m != minus_inf()) loss = loss_of(h, run.m, own.z, run.z, z, one_exp && any_entries ? z : run.z1 + own.z1);
                 }
                 if (lane == 0) a.loss[row] = loss;
             }
@@ -293,7 +296,7 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
             auto finish = [&](int n) {                       // row n of the block is done: its loss, and its record may be written again
                 wait_for(6 + (n & 3));
                 const Head &h = *record(n & 3).head;
-                const float loss = h.row_m == minus_inf() ? 0.f : loss_of(h, h.row_m, h.row_out, h.row_z, h.row_z1);
+                const float loss = h.row_m == minus_inf() ? 0.f : loss_of(h, h.row_m, h.row_in, h.row_out, h.row_z, h.row_z1);
                 if (lane == 0) a.loss[first + n * step] = loss;
             };
             Ahead ahead;
@@ -335,12 +338,12 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
             if (OWN) look_up(a, row, row + step, ahead, r);
             else i = i == RECORDS - 1 ? 0 : i + 1;
             if (!OWN && !CLUSTER) wait_for(2 + turn);
-            auto done = [&](float m, float z_out, float z, float z1) {
+            auto done = [&](float m, float z_in, float z_out, float z, float z1) {
                 if (OWN) {
-                    if (t == 0) a.loss[row] = m == minus_inf() ? 0.f : loss_of(*r.head, m, z_out, z, z1);
+                    if (t == 0) a.loss[row] = m == minus_inf() ? 0.f : loss_of(*r.head, m, z_in, z_out, z, z1);
                     __syncwarp();
                 } else if (!CLUSTER) {
-                    if (t == 0) { r.head->row_m = m; r.head->row_out = z_out; r.head->row_z = z; r.head->row_z1 = z1; }
+                    if (t == 0) { r.head->row_m = m; r.head->row_in = z_in; r.head->row_out = z_out; r.head->row_z = z; r.head->row_z1 = z1; }
                     tell(6 + turn);
                 }
             };
@@ -399,13 +402,13 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
             if (!live || run.m == minus_inf()) {           // no weight, or a mask leaves nothing of the row
                 fetch_row(row + step);
                 if (dst) for (int q = t; q < n; q += TEAM) dst[q] = 0.f;
-                done(minus_inf(), 0.f, 0.f, 0.f);
+                done(minus_inf(), 0.f, 0.f, 0.f, 0.f);
                 continue;
             }
             const float m = run.m, z_out = run.z, z = z_out + own.z, z1 = one_exp && any_entries ? z : run.z1 + own.z1;
-            if (!dst) { fetch_row(row + step); done(m, z_out, z, z1); continue; }
+            if (!dst) { fetch_row(row + step); done(m, own.z, z_out, z, z1); continue; }
             const float f_in = any_entries ? r.head->inside / z : 0.f, f_1 = ce ? (float)r.head->hard / z1 : 0.f;
-            const float f_out = tail ? (z_out > 0.f ? f_in - r.head->rest / z_out : 0.f) : f_in;
+            const float f_out = !tail ? f_in : !(z_out > 0.f) ? 0.f : own.z < 0.5f * z ? (r.head->entries - r.head->inside * (own.z / z)) / z_out : f_in - r.head->rest / z_out;
             const bool straight = misfit(dst) == off;
             // the next row's pieces follow this row's out of their places
             const bool more = row + step < a.rows;
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
                 const float d = r.head->x_label - m;
                 dst[label - c0] = f_1 * exp2_fast(d * kLog2e) + f_out * exp2_fast(d * c_t) - hard;
             }
-            done(m, z_out, z, z1);
+            done(m, own.z, z_out, z, z1);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     }

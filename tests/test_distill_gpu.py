@@ -127,6 +127,35 @@ def test_loss_and_gradient(lib, rows, cols, pad, k, T, alpha, tail):
     check(lib, wide, cols, ids, teacher, lse_of(every, T) if tail else None, labels, weights, T, alpha)
 
 
+@pytest.mark.parametrize("rows,cols,k", [(1200, 250, 1), (40, 3458, 3), (30, 8000, 2), (20, 16000, 3), (9, 70000, 4)])
+def test_entries_of_little_mass(lib, rows, cols, k):
+    """A high temperature leaves the entries P of the teacher's mass and Q of the student's, both small: the loss and the gradient outside the entries are
+    differences of the order of P and Q, and as exact as those."""
+    T = 8.0
+    rng = np.random.default_rng(cols)
+    wide, every, ids, teacher = inputs(rng, rows, cols, k, cols)
+    lse = lse_of(every, T)
+    loss, delta = run(lib, wide, cols, ids, teacher, lse, None, None, T, 0.0)
+    want, dwant, _, _ = reference(wide, ids, teacher, lse, None, None, T, 0.0)
+    at = ids.astype(np.int64)
+    x = wide.astype(D) / T
+    log_q = x - x.max(1, keepdims=True)
+    log_q -= np.log(np.exp(log_q).sum(1, keepdims=True))
+    q, log_p = np.exp(log_q), teacher.astype(D) / T - lse[:, None].astype(D)
+    P, Q = np.exp(log_p).sum(1), np.take_along_axis(q, at, 1).sum(1)
+    assert P.max() < 0.1 and Q.max() < 0.1
+    # `off` as in check(): of the sums.  Every term of the entries is p times logarithms of the size L, the two terms of the rest are ln(1 - P) and
+    # ln(1 - Q), each as exact as P and Q are.
+    off = (8 + 4 * (np.log(cols) + 1) + (cols / 32 if cols <= 256 else min(98, cols / 128)) + 4) * H
+    L = 1 + np.abs(log_p).max(1) + np.abs(np.take_along_axis(log_q, at, 1)).max(1)
+    assert np.all(np.abs(loss - want) <= T * T * off * (P * L + 2 * Q) + H * np.abs(want)), np.max(np.abs(loss - want) / (T * T * off * (P * L + 2 * Q)))
+    outside = np.ones_like(q, bool)
+    np.put_along_axis(outside, at, False, 1)
+    spread = 1 + np.abs(x - x.max(1, keepdims=True))
+    bound = T * q * (P + 2 * Q)[:, None] * (2 * off + 3 * H * spread)
+    assert np.all((np.abs(delta - dwant) <= bound)[outside]), np.max((np.abs(delta - dwant) / bound)[outside])
+
+
 @pytest.mark.parametrize("cols,k", [(20, 6), (600, 9), (5000, 40), (40000, 70)])
 @pytest.mark.parametrize("tail", [False, True])
 def test_padding_and_repeated_entries(lib, cols, k, tail):
