@@ -108,7 +108,7 @@ def draw(rng):
         rows, cols = _log_int(rng, 1, 8192), _log_int(rng, 10, 131072)
         if rows * cols <= 2 ** 27:
             tail = rng.random() < 0.4
-            return _distill(rows, cols, rng.choice([0, 0, 1, 5, 64]), min(_log_int(rng, 1, 256), cols // 2), rng.choice([0.75, 1.0, 2.0, 4.0]), rng.choice([0.0, 0.3, 0.5]), tail)
+            return _distill(rows, cols, rng.choice([0, 0, 1, 5, 64]), min(_log_int(rng, 1, 256), cols // 2), rng.choice([0.7, 1.0, 2.0, 4.0]), rng.choice([0.0, 0.3, 0.5]), tail)
 
 
 # ---- inputs ------------------------------------------------------------------------------------------------------------------
