@@ -668,15 +668,23 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
     a.unit_groups = dgate ? groups : 1;
     a.unit_rows = dgate ? (size_t)rows : total;
     // slices of a group: so many that the rounds of units over the blocks take the fewest rows one after the other
-    const size_t most = total ? with_bwd(cols, [&](auto k) { return k.resident(dev, vec, general, csize); }) : 1;
-    if (!most) return EDDLB200_ELIMIT;
     const size_t passes = total ? ceil_div(a.unit_rows, cols <= 256 ? 8 : 1) : 1;
-    size_t slices = 1, units = a.unit_groups, longest = ceil_div(units, most) * passes;
-    for (size_t rounds = 1; rounds <= 4 && a.unit_groups; rounds++) {
-        size_t s = rounds * most / a.unit_groups;
-        if (s > passes) s = passes;
-        if (s > 1 && rounds * ceil_div(passes, s) < longest) { slices = s; units = s * a.unit_groups; longest = rounds * ceil_div(passes, s); }
-    }
+    size_t most = 1, slices = 1, units = 1;
+    auto plan = [&]() {
+        most = total ? with_bwd(cols, [&](auto k) { return k.resident(dev, vec, general, csize); }) : 1;
+        if (!most) return;
+        slices = 1; units = a.unit_groups;
+        size_t longest = ceil_div(units, most) * passes;
+        for (size_t rounds = 1; rounds <= 4 && a.unit_groups; rounds++) {
+            size_t s = rounds * most / a.unit_groups;
+            if (s > passes) s = passes;
+            if (s > 1 && rounds * ceil_div(passes, s) < longest) { slices = s; units = s * a.unit_groups; longest = rounds * ceil_div(passes, s); }
+        }
+    };
+    plan();
+    // a group in one slice: a block of one team writes its dgate itself, as it holds its columns
+    if (vec && dgate && slices == 1 && cols > 256 && !aligned16(dgate)) { vec = false; plan(); }
+    if (!most) return EDDLB200_ELIMIT;
     a.slices = (int)slices;
     a.workers = (int)(units < most ? units : most);
     const size_t param_floats = a.want_param ? (size_t)a.workers * 4 * cols : 0, gate_floats = dgate && slices > 1 ? units * cols : 0;

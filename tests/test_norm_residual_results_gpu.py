@@ -1,0 +1,53 @@
+"""The backward pass of the residual norms for every choice of wanted results, with results and inputs off the 16-byte grid."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from eddl_b200.capi import DeviceArray
+from tests import test_norm_residual_gpu as base
+
+pytestmark = pytest.mark.gpu
+F = np.float32
+
+
+class Piece(DeviceArray):
+    """A tensor that begins 4 bytes behind a 16-byte border, as a piece of one flat buffer does; what lies around it has to stay."""
+
+    def __init__(self, lib, arr):
+        arr = np.ascontiguousarray(arr, dtype=F)
+        self.lib, self.dev, self.shape, self.size, self.dtype = lib, 0, arr.shape, arr.size, arr.dtype
+        self.room = lib.to_device(np.concatenate([np.full(1, 5, F), arr.ravel(), np.full(7, 5, F)]))
+        self.addr = self.room.addr + 4
+        self.ptr = ctypes.c_void_p(self.addr)
+
+    def numpy(self):
+        around = np.delete(self.room.numpy(), np.s_[1:1 + self.size])
+        assert np.all(around == 5)
+        return super().numpy()
+
+    def __del__(self):
+        pass
+
+
+class Pieces:
+    """The library as the base tests use it; tensors made after `after` calls of the forward pass are pieces."""
+
+    def __init__(self, lib, after):
+        self.lib, self.empty, self.left = lib, lib.empty, after
+
+    def call(self, name, *args):
+        self.lib.call(name, *args)
+        self.left -= name == "norm_residual_fwd"
+
+    def to_device(self, arr):
+        return self.lib.to_device(arr) if self.left > 0 else Piece(self.lib, arr)
+
+
+# one slice a group: a block writes dgate itself
+@pytest.mark.parametrize("dims", [(1, 1, 300), (1, 1, 512), (3, 1, 768), (700, 1, 512), (5, 1, 1028), (2, 1, 1400), (1, 1, 2048), (1, 1, 2304), (2, 1, 4096), (3, 1, 4500), (1, 1, 16384)])
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("inc_g", [0, 1])
+def test_dgate_off_the_grid(lib, monkeypatch, dims, kind, inc_g):
+    monkeypatch.setattr(base, "wanted", lambda c: ["dgate", "dg2"])
+    base.check(Pieces(lib, 1), base.Case(31, *dims, kind, beta=bool(kind)), inc_g=inc_g)
