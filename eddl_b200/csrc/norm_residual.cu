@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, BWD_THREADS / (TPR == 3
     extern __shared__ __align__(16) float staged[];                    // [team][2][dh, dr_out, r_out, f][SPAN]; at a unit's end the column sums of the teams
     __shared__ __align__(16) float sums[2 * K * (TPR / 32)];
     __shared__ __align__(16) float peers[CLUSTER ? 2 * K * kMaxCluster : 4];
+    if (CLUSTER) cg::this_cluster().sync();                 // the other blocks have started: their shared memory may be written
     EB_GRID_WAIT();
     TeamSum<TPR, K> sum(sums);
     const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0, csize = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;

@@ -51,3 +51,20 @@ class Pieces:
 def test_dgate_off_the_grid(lib, monkeypatch, dims, kind, inc_g):
     monkeypatch.setattr(base, "wanted", lambda c: ["dgate", "dg2"])
     base.check(Pieces(lib, 1), base.Case(31, *dims, kind, beta=bool(kind)), inc_g=inc_g)
+
+
+# the blocks of a cluster write into one another's memory with their first row: as soon as they are there (nothing to read but one gradient), and
+# more clusters than the device holds
+@pytest.mark.parametrize("dims", [(1, 1, 4097), (1, 2, 16384), (200, 1, 6000)])
+@pytest.mark.parametrize("kind", [0, 1])
+def test_first_exchange_of_a_cluster(lib, dims, kind):
+    c = base.Case(32, *dims, kind).forward()
+    dev = base.Device(lib, c).forward()
+    c.backward(dh=False)
+    got = []
+    for _ in range(20):
+        out = {"df": lib.empty(c.f.shape), "dr": lib.empty(c.r.shape)}
+        dev.backward(out, dh=None)
+        got.append([out[k].numpy() for k in ("df", "dr")])
+    assert all(np.array_equal(a, b) for g in got for a, b in zip(g, got[0]))
+    base.check(lib, c, dh=False)
