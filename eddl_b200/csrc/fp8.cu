@@ -621,6 +621,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
                     for (int i = 0; i < COLS; i++, dst += P.p_rows) if (i < columns) *dst = P.inc ? *dst + acc[i] : acc[i];
                 }
             }
+            // with an odd number of K-blocks the next tile's first scales take the place of this tile's last ones
+            if (VEC) __syncwarp();
         };
         for (int job = pair; job < jobs && !fail; job += pairs) {
             if (!HALVES || job < whole) tile(std::integral_constant<int, 64>(), job);
