@@ -657,7 +657,7 @@ int eddlb200_norm_residual_bwd(int dev, int kind, int post, int groups, int rows
         EB_REQUIRE(!(o < 2 && inc_d && out[o]) || (out[o] != dh && out[o] != dr_out && out[o] != f && out[o] != r_out), kBwd);
     }
     EB_CTX(dev);
-    const bool cluster = cols > 4096, general = kind || db1 || db2;
+    const bool cluster = cols > 4096, general = kind || db1 || db2 || (dgate && b1);        // dgate with a shift takes the sums of u too
     const unsigned csize = cluster ? (unsigned)ceil_div(cols, 2048) : 1;
     bool vec = cols % 4 == 0;
     for (int i = 0; i < 8; i++) vec = vec && aligned16(in[i]);

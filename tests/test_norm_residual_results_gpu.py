@@ -68,3 +68,15 @@ def test_first_exchange_of_a_cluster(lib, dims, kind):
         got.append([out[k].numpy() for k in ("df", "dr")])
     assert all(np.array_equal(a, b) for g in got for a, b in zip(g, got[0]))
     base.check(lib, c, dh=False)
+
+
+DIMS = [(3, 5, 96), (2, 33, 256), (2, 30, 512), (3, 4, 768), (2, 6, 1024), (2, 9, 1400), (4, 3, 2048), (2, 41, 2304), (2, 3, 4096), (2, 3, 4500), (2, 300, 6148),
+        (3, 5, 97), (40, 1, 130), (2, 9, 701), (1, 1300, 700), (2, 3, 2303), (2, 3, 5001)]
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("wanted", [["dgate"], ["df", "dr", "dgate", "dg1", "dg2"]])
+def test_dgate_with_a_shift_that_is_not_trained(lib, monkeypatch, dims, wanted):
+    """RMS norms, b1 given, neither db1 nor db2 wanted: dgate is the sum of u (n1 g1 + b1) all the same."""
+    monkeypatch.setattr(base, "wanted", lambda c: wanted)
+    base.check(lib, base.Case(33, *dims, 0, beta=True))
