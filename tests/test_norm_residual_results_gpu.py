@@ -80,3 +80,30 @@ def test_dgate_with_a_shift_that_is_not_trained(lib, monkeypatch, dims, wanted):
     """RMS norms, b1 given, neither db1 nor db2 wanted: dgate is the sum of u (n1 g1 + b1) all the same."""
     monkeypatch.setattr(base, "wanted", lambda c: wanted)
     base.check(lib, base.Case(33, *dims, 0, beta=True))
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("wanted", [["df", "dr"], ["dgate"], ["df", "dr", "dgate", "dg1", "dg2"]])
+@pytest.mark.parametrize("beta", [False, True])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_rms_norms_without_gradients_of_shifts(lib, monkeypatch, dims, wanted, beta, aligned):
+    """What a net of RMS norms without trained shifts asks for: three sums a row instead of eight."""
+    monkeypatch.setattr(base, "wanted", lambda c: wanted)
+    base.check(lib if aligned else Pieces(lib, 0), base.Case(34, *dims, 0, beta=beta))
+
+
+@pytest.mark.parametrize("dims", [(3, 5, 96), (2, 30, 512), (2, 9, 1400), (2, 3, 4500)])
+@pytest.mark.parametrize("wanted", [["dr"], ["dr", "dg2"]])
+def test_add_and_rms_norm(lib, monkeypatch, dims, wanted):
+    """r + f and its RMS norm, no gate, no norm of f; and the first norm of a net."""
+    monkeypatch.setattr(base, "wanted", lambda c: wanted + ["df"] * (c.f is not None))
+    for block in (True, False):
+        base.check(lib, base.Case(35, *dims, 0, post=0, gate=False, beta=False, block=block, scale=1.0), dr_out=block)
+        base.check(Pieces(lib, 0), base.Case(36, *dims, 0, post=0, gate=False, beta=False, block=block, scale=1.0), inc_d=1)
+
+
+@pytest.mark.parametrize("dims", DIMS)
+@pytest.mark.parametrize("kind", [0, 1])
+def test_tensors_off_the_grid(lib, dims, kind):
+    """Every tensor 4 bytes behind a 16-byte border, columns in fours or not, all gradients."""
+    base.check(Pieces(lib, 0), base.Case(37, *dims, kind))
