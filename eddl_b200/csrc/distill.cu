@@ -11,7 +11,8 @@
 // pieces in the blocks of a cluster.  What has to do with the entries (a few dozen a row: look-ups, repeated ids, 64-bit
 // exponentials) is a chain of latencies as long as the streaming of the row, so it has a warp of its own that works ahead; the
 // other warps keep a running maximum and sum a thread and meet once a row.  Mass outside the entries is summed from the
-// values outside, not as 1 minus something: with `teacher_lse` the entries' cells are set to -infinity before the sum.
+// values outside, not as 1 minus something: with `teacher_lse` the entries' cells are set to -infinity before the sum.  It stays relative to
+// the largest logit outside where that lies far below the entries': a sure student has less there than fp32 holds beside 1.
 #include <type_traits>
 #include <cooperative_groups.h>
 #include "common.cuh"
@@ -53,7 +54,8 @@ template <int HOW>
 __device__ __forceinline__ float plain(float d, float e) { return HOW == kSquare ? e * e : HOW == kFourth ? (e * e) * (e * e) : exp2_fast(d * kLog2e); }
 
 // What a row's entries and its label add.  loss = base + per_z ((m - anchor) / T + ln z) - per_rest (ln z_out - ln z) + hard (m - x_label + ln z_1), with
-// m the row's largest logit, z and z_1 the sums of exp((x - m) / T) and exp(x - m), z_out the first one outside the entries; the gradient is
+// m the row's largest logit, z and z_1 the sums of exp((x - m) / T) and exp(x - m), z_out the first one outside the entries (and (m_out - m) / T added
+// to its logarithm where it is relative to m_out, the largest logit outside); the gradient is
 // inside / z - rest / z_out times the exponential outside the entries, inside / z times it minus `less` at an entry.  Where the entries hold less than half
 // of the student's mass, z_in / z, the logarithm of z_out / z and that difference come from z_in / z: (entries - inside z_in / z) / z_out; what is
 // left of them after subtracting numbers near 1 would be good to a few digits only.
@@ -61,7 +63,7 @@ struct Head {
     double base, per_z, per_rest, hard;
     float inside, rest, entries, x_label, anchor;         // anchor: the largest of the entries' logits
     float z, z1;                                 // the entries' sums relative to it, where their cells are closed
-    float row_m, row_in, row_out, row_z, row_z1;         // what the other warps found of the row: m, z_in, z_out, z, z_1; m = -infinity: nothing that counts
+    float row_m, row_m_out, row_in, row_out, row_z, row_z1;         // what the other warps found of the row: m, m_out, z_in, z_out, z, z_1; m = -infinity: nothing that counts
     int label, label_is_entry, live;
 };
 struct Record {
@@ -253,18 +255,25 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
         run.z = warp_sum(run.z); run.z1 = warp_sum(run.z1);
         return run;
     };
-    auto add_entries = [&](Run &run, const Head &h) {
+    // The row's sums with the entries' own.  Where the largest logit outside is 2^-32 of the row's largest or less, after the temperature, the sum outside
+    // stays relative to it: beside the row's largest those classes would be zero from 2^-126 on.
+    struct Sums { float m, m_out, in, out, z, z1; };
+    auto with_entries = [&](Run run, const Head &h) {
         Run own{h.anchor, h.z, h.z1};
         if (!tail || h.z == 0.f) own.m = minus_inf();
         const float top = max_nan(run.m, own.m);
+        const bool far = tail && run.m > minus_inf() && (top - run.m) * c_t > 32.f;
+        Sums s{top, far ? run.m : top, 0.f, run.z, 0.f, 0.f};
         run.meet(top, c_t); own.meet(top, c_t);
-        return own;
+        s.in = own.z; s.z = run.z + own.z; s.z1 = one_exp && any_entries ? s.z : run.z1 + own.z1;
+        if (!far) s.out = run.z;
+        return s;
     };
-    auto loss_of = [&](const Head &h, float m, float z_in, float z_out, float z, float z1) {
+    auto loss_of = [&](const Head &h, const Sums &s) {
         double l = h.base;
-        if (any_entries) l += h.per_z * (((double)m - (double)h.anchor) / (double)a.temperature + (double)logf(z));
-        if (h.per_rest > 0.0) l -= h.per_rest * (double)(z_in < 0.5f * z ? log1pf(-z_in / z) : logf(z_out / z));
-        if (h.label >= 0) l += h.hard * ((double)m - (double)h.x_label + (double)logf(z1));
+        if (any_entries) l += h.per_z * (((double)s.m - (double)h.anchor) / (double)a.temperature + (double)logf(s.z));
+        if (h.per_rest > 0.0) l -= h.per_rest * (s.in < 0.5f * s.z ? (double)log1pf(-s.in / s.z) : (double)logf(s.out / s.z) + (s.m_out < s.m ? ((double)s.m_out - (double)s.m) / (double)a.temperature : 0.0));
+        if (h.label >= 0) l += h.hard * ((double)s.m - (double)h.x_label + (double)logf(s.z1));
         return (float)l;
     };
 
@@ -285,10 +294,8 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
                 if (rank) continue;
                 float loss = 0.f;
                 if (h.live) {
-                    Run run = combine(flip);
-                    const Run own = add_entries(run, h);
-                    const float z = run.z + own.z;
-                    if (run.m != minus_inf()) loss = loss_of(h, run.m, own.z, run.z, z, one_exp && any_entries ? z : run.z1 + own.z1);
+                    const Sums s = with_entries(combine(flip), h);
+                    if (s.m != minus_inf()) loss = loss_of(h, s);
                 }
                 if (lane == 0) a.loss[row] = loss;
             }
@@ -296,7 +303,7 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
             auto finish = [&](int n) {                       // row n of the block is done: its loss, and its record may be written again
                 wait_for(6 + (n & 3));
                 const Head &h = *record(n & 3).head;
-                const float loss = h.row_m == minus_inf() ? 0.f : loss_of(h, h.row_m, h.row_in, h.row_out, h.row_z, h.row_z1);
+                const float loss = h.row_m == minus_inf() ? 0.f : loss_of(h, Sums{h.row_m, h.row_m_out, h.row_in, h.row_out, h.row_z, h.row_z1});
                 if (lane == 0) a.loss[first + n * step] = loss;
             };
             Ahead ahead;
@@ -338,12 +345,12 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
             if (OWN) look_up(a, row, row + step, ahead, r);
             else i = i == RECORDS - 1 ? 0 : i + 1;
             if (!OWN && !CLUSTER) wait_for(2 + turn);
-            auto done = [&](float m, float z_in, float z_out, float z, float z1) {
+            auto done = [&](const Sums &s) {
                 if (OWN) {
-                    if (t == 0) a.loss[row] = m == minus_inf() ? 0.f : loss_of(*r.head, m, z_in, z_out, z, z1);
+                    if (t == 0) a.loss[row] = s.m == minus_inf() ? 0.f : loss_of(*r.head, s);
                     __syncwarp();
                 } else if (!CLUSTER) {
-                    if (t == 0) { r.head->row_m = m; r.head->row_in = z_in; r.head->row_out = z_out; r.head->row_z = z; r.head->row_z1 = z1; }
+                    if (t == 0) { r.head->row_m = s.m; r.head->row_m_out = s.m_out; r.head->row_in = s.in; r.head->row_out = s.out; r.head->row_z = s.z; r.head->row_z1 = s.z1; }
                     tell(6 + turn);
                 }
             };
@@ -397,18 +404,20 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
                 if (CLUSTER) meeting(); else team_barrier();
                 if (live) run = combine(flip);
             }
-            Run own{};
-            if (live) own = add_entries(run, *r.head);
-            if (!live || run.m == minus_inf()) {           // no weight, or a mask leaves nothing of the row
+            Sums sums{minus_inf(), 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (live) sums = with_entries(run, *r.head);
+            if (sums.m == minus_inf()) {                   // no weight, or a mask leaves nothing of the row
                 fetch_row(row + step);
                 if (dst) for (int q = t; q < n; q += TEAM) dst[q] = 0.f;
-                done(minus_inf(), 0.f, 0.f, 0.f, 0.f);
+                done(sums);
                 continue;
             }
-            const float m = run.m, z_out = run.z, z = z_out + own.z, z1 = one_exp && any_entries ? z : run.z1 + own.z1;
-            if (!dst) { fetch_row(row + step); done(m, own.z, z_out, z, z1); continue; }
-            const float f_in = any_entries ? r.head->inside / z : 0.f, f_1 = ce ? (float)r.head->hard / z1 : 0.f;
-            const float f_out = !tail ? f_in : !(z_out > 0.f) ? 0.f : own.z < 0.5f * z ? (r.head->entries - r.head->inside * (own.z / z)) / z_out : f_in - r.head->rest / z_out;
+            if (!dst) { fetch_row(row + step); done(sums); continue; }
+            const float m = sums.m, m_out = sums.m_out;
+            const bool far = tail && m_out < m;
+            const float f_in = any_entries ? r.head->inside / sums.z : 0.f, f_1 = ce ? (float)r.head->hard / sums.z1 : 0.f;
+            const float f_out = !tail ? f_in : !(sums.out > 0.f) ? 0.f : sums.in < 0.5f * sums.z ? (r.head->entries - r.head->inside * (sums.in / sums.z)) / sums.out
+                              : (far ? f_in * exp2_fast((m_out - m) * c_t) : f_in) - r.head->rest / sums.out;
             const bool straight = misfit(dst) == off;
             // the next row's pieces follow this row's out of their places
             const bool more = row + step < a.rows;
@@ -419,13 +428,13 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
                 for (int v = t; v < nv; v += TEAM) {
                     const int u = v * 4;
                     const float4 q = *reinterpret_cast<const float4 *>(x + u);
-                    const float d[4] = {q.x - m, q.y - m, q.z - m, q.w - m};
+                    const float v4[4] = {q.x, q.y, q.z, q.w};
                     float g[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float x = exp2_fast(d[e] * (decltype(want_t)::value ? c_t : kLog2e));
+                        const float x = exp2_fast((v4[e] - m_out) * (decltype(want_t)::value ? c_t : kLog2e));
                         g[e] = f * x;
-                        if (decltype(want_1)::value != kNoExp) g[e] = fmaf(f_1, plain<decltype(want_1)::value>(d[e], x), g[e]);
+                        if (decltype(want_1)::value != kNoExp) g[e] = fmaf(f_1, plain<decltype(want_1)::value>(v4[e] - m, x), g[e]);
                     }
                     if (straight && u >= off && u + 4 <= end) *reinterpret_cast<float4 *>(dst - off + u) = make_float4(g[0], g[1], g[2], g[3]);
                     else {
@@ -435,8 +444,9 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
                     if (u < next_end) fetch(next, next_off, next_end, v);
                 }
             };
-            if (any_entries && ce && !one_exp) {
-                if (a.temperature == 2.f) put(std::true_type(), Exp<kSquare>(), f_out);
+            if (any_entries && (far || (ce && !one_exp))) {
+                if (far) put(std::true_type(), Exp<kOwnExp>(), f_out);
+                else if (a.temperature == 2.f) put(std::true_type(), Exp<kSquare>(), f_out);
                 else if (a.temperature == 4.f) put(std::true_type(), Exp<kFourth>(), f_out);
                 else put(std::true_type(), Exp<kOwnExp>(), f_out);
             } else if (any_entries) put(std::true_type(), Exp<kNoExp>(), f_out + f_1);
@@ -456,9 +466,9 @@ __global__ void __launch_bounds__(block_of(TEAM, CLUSTER), blocks_per_sm(TEAM)) 
                 }
             if (ce && t == 0 && label >= c0 && label < c0 + n && !r.head->label_is_entry) {
                 const float d = r.head->x_label - m;
-                dst[label - c0] = f_1 * exp2_fast(d * kLog2e) + f_out * exp2_fast(d * c_t) - hard;
+                dst[label - c0] = f_1 * exp2_fast(d * kLog2e) + f_out * exp2_fast((r.head->x_label - m_out) * c_t) - hard;
             }
-            done(m, own.z, z_out, z, z1);
+            done(sums);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     }
