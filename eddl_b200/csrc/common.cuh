@@ -28,6 +28,9 @@ cudaEvent_t handoff_event(DevCtx *c);
 void *scratch(DevCtx *c, size_t bytes);
 // Pinned host words + device words used to return scalars (loss, accuracy).
 float *host_scalars(DevCtx *c);    // 64 floats
+// Time-out flag of the 8-bit products: a pinned word (the last of those) that a kernel writes only when it has given up waiting, so that
+// whoever waits for the device reads it without a copy.  0 = none has since it was last cleared.
+volatile int *fp8_status(DevCtx *c);
 float *dev_scalars(DevCtx *c);     // kDevScalars floats
 constexpr int kDevScalars = 1024;
 // `count` device words that are zero whenever no kernel is using them: a kernel whose blocks count their arrivals in them (the last
@@ -41,8 +44,6 @@ ncclComm *comm_of(DevCtx *c);
 int comm_nranks(DevCtx *c);
 void count_launch(DevCtx *c, unsigned n = 1);
 int set_error(int code, const char *fmt, ...);
-// Reads and clears the device's time-out flag of the 8-bit products (blocking; nothing is read on a device that has run none).
-int fp8_status(int dev, cudaStream_t st, int *out);
 
 // Optional per-kernel-family device timing (CUDA events on the compute stream), off by
 // default.  `work` is the family's algorithmic work of this call (FLOPs or bytes).

@@ -170,15 +170,12 @@ struct ProdParams {
     CUtensorMap map_p, map_q;
     const float *scale_p, *scale_q;
     float *c;
+    volatile int *status;                    // site of a wait that gave up | warp << 8 | 6 or 7 << 16
     int p_rows, q_rows, kblocks;             // p_rows: columns of C, q_rows: rows of C
     int p_shift, q_shift, p_scales, q_scales;   // rows of a scale (log2) and scales of a K-block
     int tiles_p, splits, inc, tail;          // tail: the kernel on pairs halves that many tiles, the last ones
     unsigned idesc;
 };
-
-// site of the first wait that gave up | warp << 8 | 6 << 16; 0 = none since the last look
-__device__ int g_fp8_status;
-bool g_fp8_used[EDDLB200_MAX_DEVICES] = {};
 
 // Up to 64 rows of Q two blocks share an SM: the chain copy -> MMA -> epilogue of one K-block is long and its work short, so what counts is how many
 // K-blocks are on their way (tensor memory holds BUFS of them a block).
@@ -348,7 +345,7 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, ProdShape<BN>::PER_SM)
             for (int i = 0; i < S::COLS; i++) part[i * 128] = acc[i];
         }
     }
-    if (fail) { *abort_flag = 1; atomicCAS(&g_fp8_status, 0, fail | warp << 8 | 6 << 16); }
+    if (fail) { *abort_flag = 1; *P.status = fail | warp << 8 | 6 << 16; }
     if (P.splits > 1) {
         __syncwarp();
         cluster_arrive(); cluster_wait();
@@ -629,7 +626,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
             else if constexpr (HALVES) tile(std::integral_constant<int, 32>(), job);
         }
     }
-    if (fail) { *abort_flag = 1; atomicCAS(&g_fp8_status, 0, fail | warp << 8 | 7 << 16); }
+    if (fail) { *abort_flag = 1; *P.status = fail | warp << 8 | 7 << 16; }
     tc_fence_before();
     __syncthreads();
     // both CTAs are done with each other's barriers, shared memory and accumulators
@@ -648,7 +645,6 @@ int launch_large(DevCtx *cx, int dev, cudaStream_t st, const ProdParams &P) {
     const int jobs = P.tiles_p * P.splits + P.tail, pairs = jobs < EDDLB200_NUM_SMS / 2 ? jobs : EDDLB200_NUM_SMS / 2;
     eb::launch(fp8_product_large_kernel<VEC, ROWS, HALVES>, 2 * pairs, LG_THREADS, LG_SMEM, st, P);
     EB_LAUNCH_CHECK("fp8_mult2d");
-    g_fp8_used[dev] = true;
     return 0;
 }
 
@@ -762,18 +758,6 @@ size_t scale_bytes(int rows, int cols, int block_rows) { return ceil_div(cols, k
 
 }  // namespace
 
-namespace eb {
-// 0 = no kernel of this file has given up waiting on the device since the last call
-int fp8_status(int dev, cudaStream_t st, int *out) {
-    *out = 0;
-    if (!g_fp8_used[dev]) return 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(out, g_fp8_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess && *out) { const int zero = 0; e = cudaMemcpyToSymbolAsync(g_fp8_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st); }
-    return e == cudaSuccess ? 0 : (int)e;
-}
-}  // namespace eb
-
 using namespace eb;
 
 extern "C" {
@@ -835,7 +819,7 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     EB_CTX(dev);
     if (!m || !n) return 0;
     ProdParams P;
-    P.c = c; P.kblocks = (int)ceil_div(k, kBlk);
+    P.c = c; P.status = fp8_status(cx); P.kblocks = (int)ceil_div(k, kBlk);
     struct Side { const void *q; size_t ld; const float *scale; int rows, block, format; };
     const Side sa{qa, lda, scale_a, m, block_a, format_a}, sb{qb, ldb, scale_b, n, block_b, format_b};
     auto sides = [&](const Side &p, const Side &q, int p_box, int q_box) {
@@ -872,7 +856,6 @@ int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_
     P.inc = inc_c != 0;
     ProfScope prof(cx, PROF_GEMM, 2.0 * m * n * k);
     if (!k) return inc_c ? 0 : launch_zero_fill(cx, st, c, (size_t)m * n);
-    g_fp8_used[dev] = true;
     if (!plan.bn)
         return P.tail ? large_product<true>(cx, dev, st, P, block_a, block_b) : large_product<false>(cx, dev, st, P, block_a, block_b);
     switch (plan.bn) {

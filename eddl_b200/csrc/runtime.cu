@@ -95,6 +95,7 @@ static int init_locked(int dev) {
     if ((e = cudaSetDevice(dev)) != cudaSuccess) return cuda_status(e, "cudaSetDevice");
     if ((e = cudaStreamCreateWithFlags(&c.stream, cudaStreamNonBlocking)) != cudaSuccess) return cuda_status(e, "cudaStreamCreate");
     if ((e = cudaMallocHost((void **)&c.h_scalars, 64 * sizeof(float))) != cudaSuccess) return cuda_status(e, "cudaMallocHost");
+    memset(c.h_scalars, 0, 64 * sizeof(float));
     if ((e = cudaMalloc((void **)&c.d_scalars, kDevScalars * sizeof(float))) != cudaSuccess) return cuda_status(e, "cudaMalloc");
     for (int i = 0; i < 16; i++) { cudaEventCreate(&c.ev_start[i]); cudaEventCreate(&c.ev_stop[i]); }
     if ((e = cudaEventCreateWithFlags(&c.ev_handoff, cudaEventDisableTiming)) != cudaSuccess) return cuda_status(e, "cudaEventCreate");
@@ -119,6 +120,7 @@ DevCtx *ctx_peek(int dev) { return (dev >= 0 && dev < EDDLB200_MAX_DEVICES && g_
 cudaStream_t stream_of(DevCtx *c) { return c->stream; }
 cudaEvent_t handoff_event(DevCtx *c) { return c->ev_handoff; }
 float *host_scalars(DevCtx *c) { return c->h_scalars; }
+volatile int *fp8_status(DevCtx *c) { return (volatile int *)c->h_scalars + 63; }
 float *dev_scalars(DevCtx *c) { return c->d_scalars; }
 ncclComm *comm_of(DevCtx *c) { return c->comm; }
 int comm_nranks(DevCtx *c) { return c->nranks; }
@@ -567,7 +569,7 @@ int eddlb200_sync(int dev) {
     int flag = 0;
     if (int r = conv_tc_status(dev, st, &flag)) return cuda_status((cudaError_t)r, "eddlb200_sync");
     if (flag) return set_error(EDDLB200_ETIMEOUT, "a tensor-core convolution kernel gave up waiting on a pipeline barrier (site %d, warp %d, variant 0x%x)", flag & 0xff, (flag >> 8) & 0xff, flag >> 16);
-    if (int r = fp8_status(dev, st, &flag)) return cuda_status((cudaError_t)r, "eddlb200_sync");
+    if ((flag = *fp8_status(cx))) *fp8_status(cx) = 0;
     if (flag) return set_error(EDDLB200_ETIMEOUT, "an 8-bit product gave up waiting on a pipeline barrier (site %d, warp %d, variant 0x%x)", flag & 0xff, (flag >> 8) & 0xff, flag >> 16);
     return 0;
 }
