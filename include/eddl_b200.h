@@ -293,7 +293,9 @@ int eddlb200_fp8_quantize(int dev, const float *a, int rows, int cols, int forma
 /* C[m,n] = (inc_c ? C : 0) + sum over blocks b of 128 columns: scale_a[b][row's block] * scale_b[b][row's block] * sum_{k in b} qa[m,k] qb[n,k].
  * Both operands are stored with k along their rows.  A dense layer y = x w^T is this product of x and w; its input gradient that of dy
  * and the transposed w; its weight gradient that of the transposed dy and the transposed x.  Products and sums of a block are those of
- * the tensor cores with fp32 accumulators, blocks are scaled and added in fp32; the order is fixed.  block_a, block_b: 1 or 128 rows. */
+ * the tensor cores with fp32 accumulators, blocks are scaled and added in fp32; the order is fixed.  The product of a block's two scales may be
+ * formed first, in fp32, and has to be a normal number of it (a sum of 0 times a product that overflows is a NaN, one that underflows loses
+ * digits): whether it is formed depends on the sizes.  block_a, block_b: 1 or 128 rows. */
 int eddlb200_fp8_mult2d(int dev, const void *qa, size_t lda, const float *scale_a, int format_a, int block_a,
                         const void *qb, size_t ldb, const float *scale_b, int format_b, int block_b,
                         float *c, int inc_c, int m, int n, int k);
