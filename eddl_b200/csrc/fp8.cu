@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(ProdShape<BN>::THREADS, ProdShape<BN>::PER_SM)
 // K-block moves 32 KB into each shared memory and is four instructions of 256 x 256 x 32 into one of two buffers of tensor memory.  Sixteen
 // epilogue warps, 32 lanes and 64 columns each, take a buffer out, scale it and add it to fp32 sums in registers while the next K-block
 // runs into the other one: four warps a scheduler hide the latencies between them (with eight warps of 128 columns the MMAs waited, 645 us).
-// What bounds it is power and operand traffic: 8192 x 8192 x 8192 takes 600 us, the GPU at its 1000 W and 1.5 GHz; the MMAs alone on operands that
-// are not copied 366 us at the same power, with the copies (64 KB a pair and K-block out of L2, 9 TB/s) 485.
+// What bounds it is power and operand traffic: 8192 x 8192 x 8192 takes 600 to 625 us on a layer's values, the GPU at its 1000 W and 1.5 GHz (500 on codes
+// of one sign); the MMAs alone on operands that are not copied 366 us at the same power, with the copies (64 KB a pair and K-block out of L2, 9 TB/s) 485.
 // Which operand is P is chosen so that scaling costs least: a matrix with a scale for 128 rows goes to the N side, where a warp's columns
 // share it, and an element takes one multiply-add; with a scale for every row on both sides the N side's are read from shared memory.
 // C's rows are P's rows here (ROWS) or Q's; in the first case a warp's values are turned through shared memory on their way out.
@@ -439,7 +439,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LG_THREADS, 1) fp8_p
     const uint32_t rank = cluster_rank();
     const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1), kblocks = P.kblocks;
     const int tiles_p = P.tiles_p, tail = HALVES ? P.tail : 0, whole = tiles_p * P.splits - tail, jobs = whole + 2 * tail;         // splits: here the tiles along Q
-    // Tiles in bands of twelve along P, so that the pairs at work at a time share operands in L2 (8192 cubed: 600 us, in bands of eight 635).
+    // Tiles in bands of twelve along P, so that the pairs at work at a time share operands in L2 (8192 cubed: 600 us in the same run that took 635 in bands of eight).
     // The tiles of a last round that fills half of the pairs or less are worked on in halves of 128 rows of Q, job >= whole.
     auto place = [&](int job, int &p0, int &q0) {
         const int tile = !HALVES || job < whole ? job : whole + (job - whole) / 2;
